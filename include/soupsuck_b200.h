@@ -35,7 +35,8 @@ enum {
   SB_EWORKSPACE = 4    /* workspace smaller than the *_workspace_bytes query */
 };
 
-enum { SB_F16 = 0, SB_F32 = 1 };
+/* SB_BF16 is accepted where an entry says so. */
+enum { SB_F16 = 0, SB_F32 = 1, SB_BF16 = 2 };
 
 /* Library identity and error reporting. */
 int sb_abi_version(void);
@@ -314,6 +315,33 @@ int sb_unpad_pack(const void* x, int64_t batch, int64_t seq, int64_t row_bytes, 
                   int64_t rows, void* packed, void* stream);
 int sb_unpad_scatter(const void* packed, int64_t batch, int64_t seq, int64_t row_bytes, const int32_t* cu_seqlens,
                      void* out, void* stream);
+
+/* ---------------------------------------------------------------- Distillation
+ * A teacher's answers as short lists, the loss of a student against them through its
+ * frozen head, and the use of such a student as a draft model.  No counterpart in the
+ * reference.
+ *
+ * sb_top_logits: per row of logits [rows, v] (dtype SB_F16, SB_BF16 or SB_F32; row
+ *   stride in elements, unit column stride, any alignment) the k largest values in
+ *   falling order (equal values by the lower index, NaN above +inf) in the logits'
+ *   dtype, their int64 column indices, both [rows, k], and
+ *   lse[rows] = log sum exp(logits / temperature).  1 <= k <= min(v, 256). */
+int sb_top_logits(const void* logits, int dtype, int64_t rows, int64_t v, int64_t row_stride, int k,
+                  float temperature, void* values, int64_t* indices, float* lse, void* stream);
+
+/* sb_verify_drafts: target probabilities [batch, drafts + 1, v] and draft probabilities
+ *   [batch, drafts, v] (or NULL: the drafts were chosen, their distribution is one-hot) of
+ *   one dtype, with batch and row strides in elements and unit column stride; tokens and
+ *   uniforms [batch, drafts]; noise [batch, v] fp32 > 0 (draws from Exp(1)), batch stride
+ *   noise_batch; lens [batch] or NULL: how many drafts each sequence has.
+ *   accepted[b] = leading drafts with u q(x) < p(x); out_tokens[b, drafts + 1] = those
+ *   drafts, then argmax_v r_v / noise_v with r = max(p - q, 0) at the first rejected place
+ *   (p where that is zero everywhere, and after the last draft), -1 where no r_v is above
+ *   zero, then -1.  A drafted token outside [0, v) is rejected. */
+int sb_verify_drafts(const void* target, int64_t target_batch, int64_t target_row, const void* draft,
+                     int64_t draft_batch, int64_t draft_row, int dtype, int64_t batch, int64_t drafts, int64_t v,
+                     const int64_t* tokens, const float* uniforms, const float* noise, int64_t noise_batch,
+                     const int64_t* lens, int64_t* accepted, int64_t* out_tokens, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libsoupsuck_b200.so"
 
 SB_OK, SB_EINVAL, SB_ECUDA, SB_EUNSUPPORTED, SB_EWORKSPACE = 0, 1, 2, 3, 4
-SB_F16, SB_F32 = 0, 1
+SB_F16, SB_F32, SB_BF16 = 0, 1, 2
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -82,6 +82,9 @@ SIGNATURES = {
     "sb_unpad_metadata": (_I32, [_P, _I32, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
     "sb_unpad_pack": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _P, _P]),
     "sb_unpad_scatter": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P]),
+    "sb_top_logits": (_I32, [_P, _I32, _I64, _I64, _I64, _I32, _F32, _P, _P, _P, _P]),
+    "sb_verify_drafts": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _P, _P, _P, _I64,
+                                _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()
@@ -135,6 +138,12 @@ def dtype_code(dtype) -> int:
     if dtype == torch.float32:
         return SB_F32
     raise ValueError(f"unsupported dtype {dtype}")
+
+
+def wide_dtype_code(dtype) -> int:
+    """The codes of the entries that take bf16 too."""
+    import torch
+    return SB_BF16 if dtype == torch.bfloat16 else dtype_code(dtype)
 
 
 def ptr(t) -> int | None:

@@ -17,7 +17,9 @@ import numbers
 import torch
 
 HALF, SINGLE, BYTE, LONG = torch.float16, torch.float32, torch.uint8, torch.int64
+BRAIN = torch.bfloat16
 FLOATS = (HALF, SINGLE)
+WIDE_FLOATS = (HALF, BRAIN, SINGLE)
 
 
 def _names(dtypes):
