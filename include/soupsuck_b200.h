@@ -329,6 +329,34 @@ int sb_unpad_scatter(const void* packed, int64_t batch, int64_t seq, int64_t row
 int sb_top_logits(const void* logits, int dtype, int64_t rows, int64_t v, int64_t row_stride, int k,
                   float temperature, void* values, int64_t* indices, float* lse, void* stream);
 
+/* sb_distill_forward: the divergence of a student from a teacher's listed logits, through
+ *   the student's frozen head.  hidden [t, h] and weight [v, h] of one 16-bit dtype
+ *   (h % 8 == 0, 16-byte aligned); indices [t, k] int64, distinct within a row, -1 (or any
+ *   value outside [0, v)) where a row lists fewer; logits [t, k] the teacher's there;
+ *   teacher_lse [t] = log sum exp of its whole row / temperature, or NULL.  k <= 256.
+ *   With q = softmax(hidden . weight^T / temperature) and p = exp(logits / temperature -
+ *   teacher_lse), all unlisted columns in one bucket of the rest on both sides:
+ *     loss[t] = KL(p || q)   (fp32; no temperature^2 factor)
+ *     mass[t] = the student's probability of the listed columns
+ *   NULL teacher_lse: p is normalised over the list and has no rest.  Rows without a
+ *   listed column, or whose list holds no teacher probability at all, give zeros.
+ *   du [t, h] fp32 (NULL: loss only) and place [t] int32 are what sb_distill_backward
+ *   needs: d loss / d hidden of the answered rows in compact order, and each row's place
+ *   there or -1.  Where a gradient is wanted the workspace holds 16 bits per logit of up
+ *   to 4 GB worth of rows at a time, and its contents are not needed after the call.
+ * sb_distill_backward: dhidden[t, h] (dtype) = grad[i] * d loss_i / d hidden; rows without
+ *   a list get exact zeros and never touch their (possibly non-finite) grad.
+ * sb_distill_check: faults[0] = indices that are neither -1 nor in [0, v), faults[1] =
+ *   repeats within a row (device memory, two int64; does not synchronise). */
+size_t sb_distill_workspace_bytes(int64_t t, int64_t h, int64_t v, int k, int gradient);
+int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight, int64_t v, int dtype,
+                       const int64_t* indices, const void* logits, int logits_dtype, int k, const float* teacher_lse,
+                       float temperature, float* loss, float* mass, float* du, int* place, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int sb_distill_backward(const float* du, const int* place, const float* grad, int64_t t, int64_t h, void* dhidden,
+                        int dtype, void* stream);
+int sb_distill_check(const int64_t* indices, int64_t t, int k, int64_t v, int64_t* faults, void* stream);
+
 /* sb_verify_drafts: target probabilities [batch, drafts + 1, v] and draft probabilities
  *   [batch, drafts, v] (or NULL: the drafts were chosen, their distribution is one-hot) of
  *   one dtype, with batch and row strides in elements and unit column stride; tokens and

@@ -67,16 +67,19 @@ def verify_drafts(target, tokens, uniforms, noise, draft=None, lens=None):
 
 
 def distillation(hidden, weight, indices, logits, lse=None, temperature=1.0, upstream=None):
-    """(loss, mass, dhidden or None) of KL(teacher || student) in 64 bits.
+    """(loss, mass, dhidden, spread) of KL(teacher || student) in 64 bits; the last two are
+    None without `upstream`.  spread bounds dhidden's terms: sum_v |dz_v| |W_v| |upstream| / tau.
 
     The teacher's distribution: its listed tokens and, with `lse`, one bucket of all
     others; the student's: softmax(hidden . weight^T / temperature), its unlisted tokens
     in one bucket.  Rows without a listed token give zeros."""
     x = np.asarray(hidden, dtype=np.float64)
     w = np.asarray(weight, dtype=np.float64)
+    wa = np.abs(w)
     rows, vocab = x.shape[0], w.shape[0]
     loss, mass = np.zeros(rows), np.zeros(rows)
     grad = None if upstream is None else np.zeros_like(x)
+    spread = None if upstream is None else np.zeros_like(x)
     for i in range(rows):
         used = indices[i] >= 0
         cols = indices[i][used]
@@ -107,4 +110,5 @@ def distillation(hidden, weight, indices, logits, lse=None, temperature=1.0, ups
             dz[others] -= rest * np.exp(logq[others] - log_rest)
         if upstream is not None:
             grad[i] = (dz @ w) * (upstream[i] / temperature)
-    return loss, mass, grad
+            spread[i] = (np.abs(dz) @ wa) * abs(upstream[i] / temperature)
+    return loss, mass, grad, spread

@@ -83,6 +83,11 @@ SIGNATURES = {
     "sb_unpad_pack": (_I32, [_P, _I64, _I64, _I64, _P, _I64, _P, _P]),
     "sb_unpad_scatter": (_I32, [_P, _I64, _I64, _I64, _P, _P, _P]),
     "sb_top_logits": (_I32, [_P, _I32, _I64, _I64, _I64, _I32, _F32, _P, _P, _P, _P]),
+    "sb_distill_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
+    "sb_distill_forward": (_I32, [_P, _I64, _I64, _P, _I64, _I32, _P, _P, _I32, _I32, _P, _F32, _P, _P, _P, _P,
+                                  _P, _SZ, _P]),
+    "sb_distill_backward": (_I32, [_P, _P, _P, _I64, _I64, _P, _I32, _P]),
+    "sb_distill_check": (_I32, [_P, _I64, _I32, _I64, _P, _P]),
     "sb_verify_drafts": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _P, _P, _P, _I64,
                                 _P, _P, _P, _P]),
 }

@@ -1,0 +1,643 @@
+// Distillation from a teacher's listed logits through a frozen head, with its gradient.
+//
+// Row n: student logits z_v = h . W_v / tau, q = softmax(z); the teacher lists columns J
+// with logits t_j.  With its log-sum-exp L: p_j = exp(t_j / tau - L) and one bucket of all
+// other columns, p_rest = max(0, 1 - sum p_j); without: p = softmax over J, p_rest = 0.
+//
+//   loss = sum_J g(p_j, q_j) + g(p_rest, q_rest),   g(p, q) = p log(p / q) - p + q
+//   mass = sum_J q_j
+//   d loss / d z_v = q_v - p_v on J,   q_v (1 - p_rest / q_rest) elsewhere
+//
+// The -p + q terms sum to zero over both distributions; with them every term is at
+// least zero and nothing cancels where student and teacher are close.
+//
+// Forward.  prepare sorts each row's list and computes log p; rows without a listed
+// column are left out of everything else (compact).  One tensor-core launch forms the
+// logits tile by tile (dense_pair.cuh): listed ones are written out, the others leave a
+// power-of-two exponent and a sum of exponentials per row and 128 columns, and, where a
+// gradient is wanted, the exponentials themselves in 16 bits [rows, V].  merge joins them
+// per row.  The gradient does not wait for the upstream one, which only scales rows:
+// dz is the stored exponentials times a power of two per tile (exact) with the listed
+// columns written in, du = dz . W on the tensor cores, and the row's remaining factor is
+// applied to the fp32 sums.  Against forming the logits a second time this costs one
+// read and write of the 16-bit array and saves a third of the matrix work.
+// Backward.  dhidden = upstream * du, rounded once.
+#pragma once
+
+#include "dense_pair.cuh"
+#include "gemm_host.cuh"
+
+namespace sb {
+namespace distill {
+
+constexpr int kMaxList = 256;
+constexpr int kNone = 0x7fffffff;             // an unused entry of a sorted list
+constexpr int64_t kBlockBytes = int64_t(4) << 30;  // 16-bit exponentials of one row block
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <typename T> __device__ __forceinline__ float logit_at(const void* p, int64_t i);
+template <> __device__ __forceinline__ float logit_at<float>(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+template <> __device__ __forceinline__ float logit_at<__half>(const void* p, int64_t i) {
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+template <> __device__ __forceinline__ float logit_at<__nv_bfloat16>(const void* p, int64_t i) {
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// faults[0]: indices that are neither -1 nor a column; faults[1]: repeats within a row.
+__global__ void check_kernel(const int64_t* __restrict__ indices, int64_t rows, int k, int64_t v,
+                             unsigned long long* __restrict__ faults) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int64_t* list = indices + row * k;
+  unsigned long long outside = 0, repeats = 0;
+  for (int j = lane; j < k; j += 32) {
+    const int64_t c = list[j];
+    if (c < -1 || c >= v) ++outside;
+    if (c >= 0) {
+      for (int i = 0; i < j; ++i) {
+        if (list[i] == c) {
+          ++repeats;
+          break;
+        }
+      }
+    }
+  }
+  if (outside) atomicAdd(&faults[0], outside);
+  if (repeats) atomicAdd(&faults[1], repeats);
+}
+
+// One warp per row: the used entries sorted by column, log p of each, p_rest, and how
+// many are used (0 leaves the row out).  K <= 256: an entry's place is the number of
+// entries before it.
+template <typename T>
+__global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict__ indices, const void* __restrict__ logits,
+                                                      const float* __restrict__ lse, int64_t rows, int k, int64_t v,
+                                                      float inv_tau, int* __restrict__ columns, float* __restrict__ logp,
+                                                      float* __restrict__ rest, int* __restrict__ used) {
+  __shared__ int s_col[4][kMaxList];
+  __shared__ float s_t[4][kMaxList];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (row >= rows) return;
+  int* col = s_col[warp];
+  float* tv = s_t[warp];
+  int n = 0;
+  float top = -INFINITY;
+  for (int j = lane; j < k; j += 32) {
+    const int64_t c = indices[row * k + j];
+    const bool in = c >= 0 && c < v;
+    const float t = in ? logit_at<T>(logits, row * k + j) * inv_tau : -INFINITY;
+    col[j] = in ? static_cast<int>(c) : kNone;
+    tv[j] = t;
+    n += in ? 1 : 0;
+    top = t == t ? fmaxf(top, t) : INFINITY;  // a NaN keeps the row, and makes it NaN
+  }
+  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  top = warp_max(top);
+  __syncwarp();
+  // The normaliser: the teacher's, or the list's own.
+  float norm;
+  if (lse) {
+    norm = lse[row];
+    if (norm == -INFINITY) n = 0;
+  } else {
+    float s = 0.0f;
+    for (int j = lane; j < k; j += 32) s += expf(tv[j] - top);
+    norm = top + logf(warp_sum(s));
+  }
+  if (top == -INFINITY && !lse) n = 0;  // no teacher mass on the list
+  float sum = 0.0f;
+  for (int j = lane; j < k; j += 32) {
+    const int c = col[j];
+    int place = 0;
+    for (int i = 0; i < k; ++i) place += (col[i] < c || (col[i] == c && i < j)) ? 1 : 0;
+    const float lp = c == kNone ? -INFINITY : tv[j] - norm;
+    columns[row * k + place] = c;
+    logp[row * k + place] = lp;
+    if (c != kNone) sum += expf(lp);
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) {
+    const float left = 1.0f - sum;
+    rest[row] = !lse || n == v ? 0.0f : (left < 0.0f ? 0.0f : left);
+    used[row] = n;
+  }
+}
+
+// Compact order of the rows that have a list (one block; the order is the rows').
+__global__ void __launch_bounds__(1024) compact_kernel(const int* __restrict__ used, int64_t rows, int* __restrict__ source,
+                                                       int* __restrict__ place, int* __restrict__ count) {
+  __shared__ int s_warp[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  for (int64_t start = 0; start < rows; start += 1024) {
+    const int64_t i = start + threadIdx.x;
+    const bool in = i < rows && used[i] > 0;
+    const unsigned votes = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) s_warp[warp] = __popc(votes);
+    __syncthreads();
+    int mine = s_warp[lane];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, mine, o);
+      if (lane >= o) mine += up;
+    }
+    const int before = __shfl_sync(0xffffffffu, mine, (warp + 31) & 31);
+    const int total = __shfl_sync(0xffffffffu, mine, 31);
+    const int at = base + (warp ? before : 0) + __popc(votes & ((1u << lane) - 1u));
+    if (i < rows) {
+      place[i] = in ? at : -1;
+      if (in) source[at] = static_cast<int>(i);
+    }
+    base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// 32 compact rows per CTA: their hidden states gathered, and for each row and 128-column
+// tile the first list entry at or past it.
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ hidden, int64_t h,
+                                                     const int* __restrict__ source, const int* __restrict__ count,
+                                                     const int* __restrict__ columns, int k, int tiles, int64_t ld,
+                                                     uint16_t* __restrict__ out, uint16_t* __restrict__ starts,
+                                                     float* __restrict__ loss, float* __restrict__ mass,
+                                                     const int* __restrict__ used, int64_t rows) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32;
+  if (warp == 0) {  // rows left out: zero loss and mass
+    const int64_t i = c0 + lane;
+    if (i < rows && used[i] == 0) {
+      loss[i] = 0.0f;
+      mass[i] = 0.0f;
+    }
+  }
+  const int n = *count;
+  if (c0 >= n) return;
+  for (int r = warp; r < 32 && c0 + r < n; r += 8) {
+    const uint4* from = reinterpret_cast<const uint4*>(hidden + static_cast<int64_t>(source[c0 + r]) * h);
+    uint4* to = reinterpret_cast<uint4*>(out + (c0 + r) * h);
+    for (int64_t i = lane; i < h / 8; i += 32) to[i] = from[i];
+  }
+  const int64_t c = c0 + lane;
+  if (c >= n) return;
+  const int* list = columns + static_cast<int64_t>(source[c]) * k;
+  const int per = (tiles + 1 + 7) / 8;
+  const int j0 = warp * per, j1 = j0 + per < tiles + 1 ? j0 + per : tiles + 1;
+  if (j0 >= j1) return;
+  int lo = 0, hi = k;  // first entry with column >= 128 j0
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (list[mid] < static_cast<int64_t>(j0) * 128) lo = mid + 1; else hi = mid;
+  }
+  int next = lo < k ? list[lo] : kNone;
+  for (int j = j0; j < j1; ++j) {
+    while (next < static_cast<int64_t>(j) * 128) next = ++lo < k ? list[lo] : kNone;
+    // Unused entries (kNone) lie past every tile: the last start counts used ones only.
+    starts[static_cast<int64_t>(j) * ld + c] = static_cast<uint16_t>(lo);
+  }
+}
+
+// g(p, q) from logarithms: q (r e^r - e^r + 1) with r = log(p / q), by its series
+// r^2/2 + r^3/3 + r^4/8 + ... where the closed form would cancel, and as p r - p + q where
+// e^r would be large.
+__device__ __forceinline__ float gap(float p, float logp, float q, float logq) {
+  if (!(p > 0.0f) && p == p) return q;
+  const float r = logp - logq;
+  if (fabsf(r) < 0.25f) {
+    const float poly =
+        r * r * (0.5f + r * (1.0f / 3 + r * (0.125f + r * (1.0f / 30 + r * (1.0f / 144 + r * (1.0f / 840 + r * (1.0f / 5760)))))));
+    return q * poly;
+  }
+  if (r > 1.0f) return fmaf(p, r, q - p);
+  return q * (r * expf(r) - expm1f(r));
+}
+
+// Eight rows per CTA.  Joins a row's tile statistics and listed logits into its loss and
+// mass, and for the gradient: `shift` so that a tile's exponentials times 2^(M + shift)
+// are dz in the row's unit, `unit` (dz's factor), and the listed columns' dz / unit (over
+// their logits).  The unit is a power of two times the factor all unlisted columns share,
+//   b = 2^(R - lse2) - p_rest / S     (R the largest M, S the sum of 2^(y - R)),
+// so only the listed columns' values are rounded anew, and is such that neither passes
+// 2^15 in fp16.
+constexpr int kMergeThreads = 1024;
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(
+    const float2* __restrict__ stats, int64_t ld, int tiles, const int* __restrict__ count, int row_base,
+    const int* __restrict__ source, const int* __restrict__ used, const float* __restrict__ logp,
+    const float* __restrict__ rest, int k, float scale, float* __restrict__ listed, float* __restrict__ loss,
+    float* __restrict__ mass, float* __restrict__ unit, int* __restrict__ shift) {
+  __shared__ float s_r[kMergeThreads], s_s[kMergeThreads];
+  const int n = *count - row_base;
+  const int r = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + r;
+  if (static_cast<int64_t>(blockIdx.x) * 8 >= n) return;
+  float R = -1e30f, S = 0.0f;
+  if (row < n) {
+    for (int j = g; j < tiles; j += kMergeThreads / 8) {
+      const float2 t = stats[j * ld + row];
+      if (t.y == 0.0f) continue;
+      if (t.x > R) {
+        S *= exp2f(R - t.x);
+        R = t.x;
+      }
+      S += t.y * exp2f(t.x - R);  // a power of two: exact
+    }
+  }
+  s_r[threadIdx.x] = R;
+  s_s[threadIdx.x] = S;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp >= 8) return;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  if (at >= n) return;
+  R = -1e30f;
+  S = 0.0f;
+  for (int i = lane; i < kMergeThreads / 8; i += 32) R = fmaxf(R, s_r[i * 8 + warp]);
+  R = warp_max(R);
+  for (int i = lane; i < kMergeThreads / 8; i += 32) {
+    const float s = s_s[i * 8 + warp];
+    if (s != 0.0f) S += s * exp2f(s_r[i * 8 + warp] - R);
+  }
+  S = warp_sum(S) * exp2f(-dense::kLift);
+  const int64_t src = source[row_base + at];
+  const int m = used[src];
+  float* z = listed + (row_base + at) * k;
+  const float* lp = logp + src * k;
+  float top = S > 0.0f ? R : -INFINITY;
+  for (int j = lane; j < m; j += 32) top = fmaxf(top, z[j] * scale);
+  top = warp_max(top);
+  float total = 0.0f;
+  for (int j = lane; j < m; j += 32) total += exp2f(fmaf(z[j], scale, -top));
+  total = warp_sum(total);
+  if (S != 0.0f) total += S * exp2f(R - top);
+  const float lse2 = top + log2f(total);
+  float gaps = 0.0f, covered = 0.0f, largest = 0.0f;
+  for (int j = lane; j < m; j += 32) {
+    const float y = fmaf(z[j], scale, -lse2);
+    const float q = exp2f(y), p = expf(lp[j]);
+    gaps += gap(p, lp[j], q, y * kLn2);
+    covered += q;
+    const float d = q - p;
+    largest = fmaxf(largest, fabsf(d));
+    z[j] = d;
+  }
+  gaps = warp_sum(gaps);
+  covered = warp_sum(covered);
+  largest = warp_max(largest);
+  const float p_rest = rest[src];
+  const float head = exp2f(R - lse2);
+  if (lane == 0) {
+    if (S > 0.0f || !(S == S)) gaps += gap(p_rest, logf(p_rest), S * head, (R - lse2 + log2f(S)) * kLn2);
+    loss[src] = gaps;
+    mass[src] = covered;
+  }
+  if (!unit) return;
+  const float a = S == 0.0f ? 0.0f : (head - p_rest / S) * exp2f(-dense::kLift);
+  float f;
+  int e;
+  if (a == 0.0f) {
+    e = -100000;  // no unlisted share: the stored exponentials become zeros
+    f = largest > 0.0f ? exp2f(static_cast<float>(ilogbf(largest)) - dense::kLift) : 1.0f;
+  } else {
+    int down = largest > 0.0f ? 14 + ilogbf(a) - ilogbf(largest) : 0;
+    if (!(a == a) || isinf(a) || !(largest < INFINITY)) down = 0;
+    down = down > 0 ? 0 : down;
+    e = down - static_cast<int>(R);
+    f = ldexpf(a, -down);
+  }
+  for (int j = lane; j < m; j += 32) z[j] = z[j] / f;
+  if (lane == 0) {
+    unit[row_base + at] = f;
+    shift[row_base + at] = e;
+  }
+}
+
+// dz of one row's segment in place: each tile's exponentials times 2^(M + shift), then
+// the listed columns.
+constexpr int kScaleThreads = 256, kScaleVecs = 4;
+template <bool BF16>
+__global__ void __launch_bounds__(kScaleThreads) scale_kernel(
+    uint16_t* __restrict__ dz, int64_t pitch, const float2* __restrict__ stats, int64_t ld, const int* __restrict__ count,
+    int row_base, const int* __restrict__ source, const int* __restrict__ used, const int* __restrict__ columns,
+    const float* __restrict__ listed, int k, const int* __restrict__ shift) {
+  const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 32768;
+  if (row >= *count - row_base || row >= ld) return;
+  const int e = shift[row_base + row];
+  uint16_t* line = dz + row * pitch;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kScaleThreads * kScaleVecs;
+#pragma unroll
+  for (int i = 0; i < kScaleVecs; ++i) {
+    const int64_t vec = v0 + i * kScaleThreads + threadIdx.x;
+    if (vec * 8 >= pitch) break;
+    const float2 t = stats[(vec >> 4) * ld + row];
+    const int by = static_cast<int>(t.x) + e;
+    if (by == 0 || t.y == 0.0f) continue;
+    const float f = exp2f(static_cast<float>(by));
+    uint4* at = reinterpret_cast<uint4*>(line) + vec;
+    uint4 w = *at;
+    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (BF16) {
+        x[j] = dense::pack2<true>(__uint_as_float(x[j] << 16) * f, __uint_as_float(x[j] & 0xffff0000u) * f);
+      } else {
+        const float2 y = __half22float2(*reinterpret_cast<__half2*>(&x[j]));
+        x[j] = dense::pack2<false>(y.x * f, y.y * f);
+      }
+    }
+    *at = w;
+  }
+  __syncthreads();
+  const int64_t c0 = v0 * 8, c1 = c0 + kScaleThreads * kScaleVecs * 8;
+  const int64_t src = source[row_base + row];
+  const int n = used[src];
+  for (int j = threadIdx.x; j < n; j += kScaleThreads) {
+    const int c = columns[src * k + j];
+    if (c >= c0 && c < c1) {
+      line[c] = static_cast<uint16_t>(dense::pack2<BF16>(listed[(row_base + row) * k + j], 0.0f) & 0xffffu);
+    }
+  }
+}
+
+// du[compact row] = unit / tau * (sum of the splits, in their order).
+__global__ void __launch_bounds__(256) sum_kernel(const float* __restrict__ parts, int64_t h, int k_blocks, int pairs,
+                                                  int64_t room, const int* __restrict__ count, int row_base, int rows_cap,
+                                                  const float* __restrict__ unit, float inv_tau, float* __restrict__ du) {
+  const int left = *count - row_base;
+  const int rows = left < rows_cap ? left : rows_cap;
+  if (rows <= 0) return;
+  const int splits = dense::product_splits(rows, static_cast<int>(h), k_blocks, pairs, room);
+  const int64_t part = static_cast<int64_t>((rows + dense::kTile - 1) / dense::kTile * dense::kTile) * h;
+  const int64_t vecs = static_cast<int64_t>(rows) * h / 4;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < vecs;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < splits; ++s) {
+      const float4 x = reinterpret_cast<const float4*>(parts + s * part)[i];
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    }
+    const float f = unit[row_base + i * 4 / h] * inv_tau;
+    reinterpret_cast<float4*>(du + static_cast<int64_t>(row_base) * h)[i] = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+  }
+}
+
+// dhidden = grad * du for rows with a list, exact zeros for the others whatever their grad.
+template <bool BF16>
+__global__ void __launch_bounds__(256) backward_kernel(const float* __restrict__ du, const int* __restrict__ place,
+                                                       const float* __restrict__ grad, int64_t rows, int64_t h,
+                                                       uint16_t* __restrict__ out) {
+  const int64_t vecs = rows * h / 8;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < vecs;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = i * 8 / h, col = i * 8 - row * h;
+    const int c = place[row];
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (c >= 0) {
+      const float g = grad[row];
+      const float4* from = reinterpret_cast<const float4*>(du + c * h + col);
+      const float4 a = from[0], b = from[1];
+      w = make_uint4(dense::pack2<BF16>(a.x * g, a.y * g), dense::pack2<BF16>(a.z * g, a.w * g),
+                     dense::pack2<BF16>(b.x * g, b.y * g), dense::pack2<BF16>(b.z * g, b.w * g));
+    }
+    reinterpret_cast<uint4*>(out)[i] = w;
+  }
+}
+
+// ----------------------------------------------------------------- workspace
+struct Layout {
+  int64_t tiles, pitch, cap, room;
+  int n_tiles, out_tiles, k_blocks;
+  size_t columns, logp, listed, rest, used, source, count, unit, shift, hidden, starts, stats, dz, parts, total;
+};
+
+inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
+  Layout L{};
+  L.n_tiles = static_cast<int>((v + dense::kTile - 1) / dense::kTile);
+  L.tiles = 2 * static_cast<int64_t>(L.n_tiles);
+  L.pitch = (v + 63) / 64 * 64;
+  L.cap = t;
+  if (train) {
+    int64_t rows = kBlockBytes / (L.pitch * 2) / dense::kTile * dense::kTile;
+    if (rows < dense::kTile) rows = dense::kTile;
+    if (rows < t) L.cap = rows;
+  }
+  L.out_tiles = static_cast<int>((h + dense::kTile - 1) / dense::kTile);
+  L.k_blocks = static_cast<int>(L.pitch / 64);
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o = gemm::align256(o + bytes);
+    return at;
+  };
+  L.columns = take(t * k * 4);
+  L.logp = take(t * k * 4);
+  L.listed = take(t * k * 4);
+  L.rest = take(t * 4);
+  L.used = take(t * 4);
+  L.source = take(t * 4);
+  L.count = take(16);
+  L.unit = take(t * 4);
+  L.shift = take(t * 4);
+  L.hidden = take(t * h * 2);
+  L.starts = take((L.tiles + 1) * t * 2);
+  L.stats = take(L.tiles * L.cap * 8);
+  if (train) {
+    L.dz = take(L.cap * L.pitch * 2);
+    // Partial sums of the product, whose splits are chosen on the device from the
+    // answered rows: 512 MB while that holds four splits of the whole block, and no
+    // more than one split per pair of SMs can use.
+    const int64_t one = (L.cap + dense::kTile - 1) / dense::kTile * dense::kTile * h;
+    int64_t splits = (int64_t(1) << 27) / one;
+    splits = splits < 4 ? 4 : splits;
+    const int pairs = device_sm_count() / 2;
+    L.room = one * (splits < pairs ? splits : pairs);
+    L.parts = take(L.room * 4);
+  }
+  L.total = o;
+  return L;
+}
+
+template <bool BF16>
+int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, float temperature,
+            const Layout& L, uint8_t* ws, float* loss, float* mass, float* du, int* place, cudaStream_t st) {
+  using namespace gemm;
+  auto ptr = [&](size_t at) { return ws + at; };
+  int* columns = reinterpret_cast<int*>(ptr(L.columns));
+  float* logp = reinterpret_cast<float*>(ptr(L.logp));
+  float* listed = reinterpret_cast<float*>(ptr(L.listed));
+  float* rest = reinterpret_cast<float*>(ptr(L.rest));
+  int* used = reinterpret_cast<int*>(ptr(L.used));
+  int* source = reinterpret_cast<int*>(ptr(L.source));
+  int* count = reinterpret_cast<int*>(ptr(L.count));
+  float* unit = reinterpret_cast<float*>(ptr(L.unit));
+  int* shift = reinterpret_cast<int*>(ptr(L.shift));
+  uint16_t* hc = reinterpret_cast<uint16_t*>(ptr(L.hidden));
+  uint16_t* starts = reinterpret_cast<uint16_t*>(ptr(L.starts));
+  float2* stats = reinterpret_cast<float2*>(ptr(L.stats));
+  const bool train = du != nullptr;
+  uint16_t* dz = train ? reinterpret_cast<uint16_t*>(ptr(L.dz)) : nullptr;
+  float* parts = train ? reinterpret_cast<float*>(ptr(L.parts)) : nullptr;
+  const CUtensorMapDataType dt = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const float scale = kLog2e / temperature;
+  const int pairs = device_sm_count() / 2;
+
+  compact_kernel<<<1, 1024, 0, st>>>(used, t, source, place, count);
+  count_launch();
+  gather_kernel<<<static_cast<unsigned>((t + 31) / 32), 256, 0, st>>>(hidden, h, source, count, columns, k,
+                                                                       static_cast<int>(L.tiles), t, hc, starts, loss, mass,
+                                                                       used, t);
+  count_launch();
+  if (int rc = check_launch("distill compact")) return rc;
+  CUtensorMap m_w;
+  int rc = make_map(&m_w, dt, weight, h, v, h * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  for (int64_t r0 = 0; r0 < t; r0 += L.cap) {
+    const int64_t rows = t - r0 < L.cap ? t - r0 : L.cap;
+    CUtensorMap m_h, m_dz, m_dz_out, m_wn, m_parts;
+    rc = make_map(&m_h, dt, hc + r0 * h, h, rows, h * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc && train) rc = make_map(&m_dz_out, dt, dz, L.pitch, rows, L.pitch * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    dense::Params p{};
+    p.count = count;
+    p.row_base = static_cast<int>(r0);
+    p.rows_cap = static_cast<int>(rows);
+    p.cols = static_cast<int>(v);
+    p.n_tiles = L.n_tiles;
+    p.k_blocks = static_cast<int>((h + 63) / 64);
+    p.seg = 4;
+    p.scale = scale;
+    p.list = k;
+    p.columns = columns;
+    p.source = source;
+    p.starts = starts;
+    p.starts_ld = t;
+    p.listed = listed;
+    p.stats = stats;
+    p.store = train ? 1 : 0;
+    rc = dense::launch<false, BF16>(m_h, m_w, train ? m_dz_out : m_h, p, st, "distill_logits");
+    if (rc) return rc;
+    merge_kernel<<<static_cast<unsigned>((rows + 7) / 8), kMergeThreads, 0, st>>>(
+        stats, rows, static_cast<int>(L.tiles), count, static_cast<int>(r0), source, used, logp, rest, k, scale, listed, loss,
+        mass, train ? unit : nullptr, shift);
+    count_launch();
+    if (int e = check_launch("distill merge")) return e;
+    if (!train) continue;
+    const dim3 grid(static_cast<unsigned>((L.pitch / 8 + kScaleThreads * kScaleVecs - 1) / (kScaleThreads * kScaleVecs)),
+                    static_cast<unsigned>(rows < 32768 ? rows : 32768), static_cast<unsigned>((rows + 32767) / 32768));
+    scale_kernel<BF16><<<grid, kScaleThreads, 0, st>>>(dz, L.pitch, stats, rows, count, static_cast<int>(r0), source, used,
+                                                       columns, listed, k, shift);
+    count_launch();
+    if (int e = check_launch("distill scale")) return e;
+    rc = make_map(&m_dz, dt, dz, L.pitch, rows, L.pitch * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = make_map(&m_wn, dt, weight, h, v, h * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) {
+      rc = make_map(&m_parts, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, parts, h, L.room / h, h * 4, 32, 32,
+                    CU_TENSOR_MAP_SWIZZLE_128B);
+    }
+    if (rc) return rc;
+    dense::Params d{};
+    d.count = count;
+    d.row_base = static_cast<int>(r0);
+    d.rows_cap = static_cast<int>(rows);
+    d.cols = static_cast<int>(h);
+    d.n_tiles = L.out_tiles;
+    d.k_blocks = L.k_blocks;
+    d.seg = 16;
+    d.room = L.room;
+    rc = dense::launch<true, BF16>(m_dz, m_wn, m_parts, d, st, "distill_product");
+    if (rc) return rc;
+    sum_kernel<<<static_cast<unsigned>(device_sm_count() * 4), 256, 0, st>>>(
+        parts, h, L.k_blocks, pairs, L.room, count, static_cast<int>(r0), static_cast<int>(rows), unit, 1.0f / temperature, du);
+    count_launch();
+    if (int e = check_launch("distill sum")) return e;
+  }
+  return SB_OK;
+}
+
+}  // namespace distill
+}  // namespace sb
+
+extern "C" {
+
+size_t sb_distill_workspace_bytes(int64_t t, int64_t h, int64_t v, int k, int gradient) {
+  if (t <= 0 || h <= 0 || v <= 0 || k <= 0) return 0;
+  return sb::distill::layout(t, h, v, k, gradient != 0).total;
+}
+
+int sb_distill_check(const int64_t* indices, int64_t t, int k, int64_t v, int64_t* faults, void* stream) {
+  SB_REQUIRE(faults != nullptr, "NULL faults");
+  SB_REQUIRE(t >= 0 && k >= 1 && v > 0, "expected t >= 0, k >= 1, v > 0");
+  cudaStream_t st = sb::as_stream(stream);
+  cudaError_t e = cudaMemsetAsync(faults, 0, 2 * sizeof(int64_t), st);
+  if (e != cudaSuccess) return sb::fail(SB_ECUDA, cudaGetErrorString(e));
+  if (t == 0) return SB_OK;
+  SB_REQUIRE(indices != nullptr, "NULL indices");
+  SB_REQUIRE(t <= 0x7fffffff, "size out of range");
+  sb::distill::check_kernel<<<static_cast<unsigned>((t + 7) / 8), 256, 0, st>>>(indices, t, k, v,
+                                                                                reinterpret_cast<unsigned long long*>(faults));
+  sb::count_launch();
+  return sb::check_launch("distill check");
+}
+
+int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight, int64_t v, int dtype,
+                       const int64_t* indices, const void* logits, int logits_dtype, int k, const float* teacher_lse,
+                       float temperature, float* loss, float* mass, float* du, int* place, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  using namespace sb::distill;
+  SB_REQUIRE(t >= 0 && h > 0 && v > 0, "expected t >= 0, h > 0, v > 0");
+  SB_REQUIRE(dtype == SB_F16 || dtype == SB_BF16, "hidden and weight must be fp16 or bf16");
+  SB_REQUIRE(logits_dtype == SB_F16 || logits_dtype == SB_BF16 || logits_dtype == SB_F32, "logits must be fp16, bf16 or fp32");
+  SB_REQUIRE(k >= 1 && k <= kMaxList, "k must be between 1 and 256");
+  SB_REQUIRE(temperature > 0.0f && temperature < INFINITY, "temperature must be positive and finite");
+  if (t == 0) return SB_OK;
+  SB_REQUIRE(hidden && weight && indices && logits && loss && mass && place, "NULL pointer argument");
+  SB_REQUIRE(h % 8 == 0, "hidden size must be a multiple of 8 (pad with zeros)");
+  SB_REQUIRE(sb::aligned(hidden, 16) && sb::aligned(weight, 16), "operands must be 16-byte aligned");
+  SB_REQUIRE(t <= (int64_t(1) << 30) && v <= (int64_t(1) << 30) && h <= (int64_t(1) << 20), "size out of range");
+  const Layout L = layout(t, h, v, k, du != nullptr);
+  SB_REQUIRE(!du || L.room / h < 0x7fffffff, "size out of range");
+  if (!workspace || workspace_bytes < L.total) return sb::fail(SB_EWORKSPACE, "distillation workspace too small");
+  cudaStream_t st = sb::as_stream(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  auto prepare = logits_dtype == SB_F32   ? prepare_kernel<float>
+                 : logits_dtype == SB_F16 ? prepare_kernel<__half>
+                                          : prepare_kernel<__nv_bfloat16>;
+  prepare<<<static_cast<unsigned>((t + 3) / 4), 128, 0, st>>>(
+      indices, logits, teacher_lse, t, k, v, 1.0f / temperature, reinterpret_cast<int*>(ws + L.columns),
+      reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest), reinterpret_cast<int*>(ws + L.used));
+  sb::count_launch();
+  if (int rc = sb::check_launch("distill prepare")) return rc;
+  return dtype == SB_BF16
+             ? forward<true>(hidden, t, h, weight, v, k, temperature, L, ws, loss, mass, du, place, st)
+             : forward<false>(hidden, t, h, weight, v, k, temperature, L, ws, loss, mass, du, place, st);
+}
+
+int sb_distill_backward(const float* du, const int* place, const float* grad, int64_t t, int64_t h, void* dhidden, int dtype,
+                        void* stream) {
+  SB_REQUIRE(t >= 0 && h > 0 && h % 8 == 0, "expected t >= 0 and h a positive multiple of 8");
+  SB_REQUIRE(dtype == SB_F16 || dtype == SB_BF16, "dhidden must be fp16 or bf16");
+  if (t == 0) return SB_OK;
+  SB_REQUIRE(du && place && grad && dhidden, "NULL pointer argument");
+  cudaStream_t st = sb::as_stream(stream);
+  const int64_t blocks = (t * h / 8 + 255) / 256;
+  const unsigned grid = static_cast<unsigned>(blocks < sb::device_sm_count() * 8 ? blocks : sb::device_sm_count() * 8);
+  if (dtype == SB_BF16) {
+    sb::distill::backward_kernel<true><<<grid, 256, 0, st>>>(du, place, grad, t, h, static_cast<uint16_t*>(dhidden));
+  } else {
+    sb::distill::backward_kernel<false><<<grid, 256, 0, st>>>(du, place, grad, t, h, static_cast<uint16_t*>(dhidden));
+  }
+  sb::count_launch();
+  return sb::check_launch("distill backward");
+}
+
+}  // extern "C"

@@ -10,10 +10,11 @@ from .nf4_gemm import nf4_matmul, nf4_lora_linear
 from .lora_epilogue import lora_epilogue
 from .mlp import nf4_swiglu_mlp, swiglu_fused_backward, swiglu_fused_forward
 from .rope import fused_rope
+from .distillation import fused_linear_distillation
 from .top_logits import top_logits
 from .verify import verify_drafts
 
 __all__ = ["fused_linear_cross_entropy", "rms_norm", "add_rms_norm", "dequantize_nf4",
            "nf4_matmul", "nf4_lora_linear", "lora_epilogue", "nf4_swiglu_mlp",
            "swiglu_fused_forward", "swiglu_fused_backward", "fused_rope", "top_logits",
-           "verify_drafts"]
+           "fused_linear_distillation", "verify_drafts"]
