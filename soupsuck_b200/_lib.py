@@ -9,6 +9,7 @@ SB_EINVAL and RuntimeError otherwise, with the library's message.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -134,6 +135,21 @@ def query(name, *args) -> int:
 def stream_of(device) -> int:
     import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(device) -> int:
+    """stream_of without building a Stream object (2 us of a call's host time)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context with `device` current; free when it already is."""
+    import torch
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def dtype_code(dtype) -> int:

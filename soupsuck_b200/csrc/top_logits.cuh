@@ -6,22 +6,27 @@
 // tie and "the k largest" is unique: the result does not depend on the schedule.
 //
 // One pass over the row.  A CTA streams its row (or its share of one; a cluster of
-// CTAs splits a row when there are few) in 16-byte vectors:
-//   * log-sum-exp: each thread keeps a running maximum m and the sum of
-//     2^((z - m) log2(e) / tau), rescaled only when a vector's maximum passes m;
-//   * selection: elements above a threshold go to a shared-memory buffer.  The first
-//     threshold is the k-th largest of the threads' maxima over their first vectors
-//     (k different elements reach it, so nothing that belongs to the k largest is
-//     below it); whenever the buffer has passed kKeep entries at a chunk's end it is
-//     cut to its k largest and the k-th becomes the threshold, strictly, because
-//     later elements of equal value have higher indices.  A chunk adds at most its
-//     own size, so the buffer cannot overflow for any input.
-// The test costs one packed maximum per two 16-bit elements; the buffer sees a few
-// hundred elements of a row of 10^5.
+// CTAs splits a row when there are few) in 16-byte vectors, kVecs per thread and round:
+//   * log-sum-exp: each thread keeps a running maximum m and the sums of
+//     2^((z - m) log2(e) / tau), rescaled only when a round's maximum passes m;
+//   * selection: vectors with an element at or above a threshold go to a list in shared
+//     memory, which is sorted out when the row has been read.
+// The threshold is a guess.  The 32 streams of a CTA (warp, vector) lie side by side in
+// the row, so the first round is an even sample of it; with s of n elements sampled, the
+// r-th largest of the threads' maxima, r = k s / n + 2.5 sqrt(k s / n) + 3, leaves a few
+// times k candidates and almost never fewer than k.  Where it does leave fewer, or the
+// list overflows (a row of equal or masked logits), the row is read again with the
+// threshold that cannot fail: the k-th largest of the threads' maxima over a first chunk
+// in index order, raised to the k-th of all so far whenever the candidates have doubled;
+// the list then holds a whole chunk and is worked off at its end, so any row is handled.
+// 3300 rows of 151936 fp16, k = 64: reading takes 154 us, the safe form alone 259 us
+// (taking the vectors apart in the loop instead of listing them 703 us).
 #pragma once
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -30,10 +35,13 @@ namespace top {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kMaxK = 256;
-constexpr int kKeep = 2048;
-constexpr int kVecs = 2;  // 16-byte vectors per thread and chunk
+constexpr int kVecs = 4;                      // 16-byte vectors per thread and chunk
+constexpr int kChunk = kThreads * kVecs;      // vectors
+constexpr int kBuffer = 2048;
+constexpr int kRankable = 512;                // candidates that are sorted without a selection
+constexpr int kPerSm = 4;
 
 using u64 = unsigned long long;
 
@@ -53,12 +61,15 @@ template <typename T> struct Kind;
 
 template <> struct Kind<float> {
   static constexpr int kPer = 4;
+  static constexpr bool kBrain = false;
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising32(reinterpret_cast<const uint32_t*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising32(__float_as_uint(f)); }
   struct Limit { float t; };
   static __device__ __forceinline__ float value(const uint4& v, int i) {
     return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
   }
-  static __device__ __forceinline__ uint32_t key(const uint4& v, int i) {
-    return rising32(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+  static __device__ __forceinline__ float2 pair_value(const uint4& v, int i) {
+    return make_float2(value(v, 2 * i), value(v, 2 * i + 1));
   }
   static __device__ __forceinline__ uint32_t scalar_key(const float* p) { return rising32(__float_as_uint(*p)); }
   static __device__ __forceinline__ float top(const uint4& v) {
@@ -85,23 +96,19 @@ template <typename T, typename T2> struct Kind16 {
     const uint32_t w = word(v, i);
     return *reinterpret_cast<const T2*>(&w);
   }
-  static __device__ __forceinline__ uint32_t bits(const uint4& v, int i) {
-    const uint32_t w = word(v, i >> 1);
-    return (i & 1) ? w >> 16 : w & 0xffffu;
-  }
   static __device__ __forceinline__ Limit limit_of(T t) { return Limit{T2(t, t)}; }
 };
 
 template <> struct Kind<__half> : Kind16<__half, __half2> {
+  static constexpr bool kBrain = false;
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising(reinterpret_cast<const unsigned short*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising(__half_as_ushort(__float2half_rd(f))); }
   static __device__ __forceinline__ uint32_t rising(uint32_t b) {
     if ((b & 0x7fffu) == 0u) return 0x80000000u;
     if ((b & 0x7fffu) > 0x7c00u) return 0xffff0000u;
     return ((b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u)) << 16;
   }
-  static __device__ __forceinline__ float value(const uint4& v, int i) {
-    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits(v, i))));
-  }
-  static __device__ __forceinline__ uint32_t key(const uint4& v, int i) { return rising(bits(v, i)); }
+  static __device__ __forceinline__ float2 pair_value(const uint4& v, int i) { return __half22float2(pair(v, i)); }
   static __device__ __forceinline__ uint32_t scalar_key(const __half* p) { return rising(__half_as_ushort(*p)); }
   static __device__ __forceinline__ __half2 top2(const uint4& v) {
     return __hmax2_nan(__hmax2_nan(pair(v, 0), pair(v, 1)), __hmax2_nan(pair(v, 2), pair(v, 3)));
@@ -120,16 +127,18 @@ template <> struct Kind<__half> : Kind16<__half, __half2> {
 };
 
 template <> struct Kind<__nv_bfloat16> : Kind16<__nv_bfloat16, __nv_bfloat162> {
+  static constexpr bool kBrain = true;
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising(reinterpret_cast<const unsigned short*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising(__bfloat16_as_ushort(__float2bfloat16_rd(f))); }
   static __device__ __forceinline__ uint32_t rising(uint32_t b) {
     if ((b & 0x7fffu) == 0u) return 0x80000000u;
     if ((b & 0x7fffu) > 0x7f80u) return 0xffff0000u;
     return ((b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u)) << 16;
   }
-  static __device__ __forceinline__ float value(const uint4& v, int i) {
-    const uint32_t w = word(v, i >> 1);
-    return __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+  static __device__ __forceinline__ float2 pair_value(const uint4& v, int i) {
+    const uint32_t w = word(v, i);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint32_t key(const uint4& v, int i) { return rising(bits(v, i)); }
   static __device__ __forceinline__ uint32_t scalar_key(const __nv_bfloat16* p) { return rising(__bfloat16_as_ushort(*p)); }
   static __device__ __forceinline__ __nv_bfloat162 top2(const uint4& v) {
     return __hmax2_nan(__hmax2_nan(pair(v, 0), pair(v, 1)), __hmax2_nan(pair(v, 2), pair(v, 3)));
@@ -162,19 +171,17 @@ __device__ __forceinline__ u64 full_key(uint32_t key, int64_t index) {
   return (static_cast<u64>(key) << 32) | (0xffffffffull - static_cast<u64>(index));
 }
 
-template <typename T> constexpr int chunk_elems() { return kThreads * kVecs * Kind<T>::kPer; }
-// The buffer: what one chunk (and the row's unaligned ends) can add to kKeep entries.
-template <typename T> constexpr int capacity() { return kKeep + chunk_elems<T>() + 32; }
-
 struct Scratch {
-  int hist[256];
-  int count;    // entries in the buffer
-  int picked;   // entries of the selection below
-  int digit, need;
-  float warp_m[kThreads / 32], warp_s[kThreads / 32];
-  float m, s;   // this CTA's log-sum-exp parts
-  int out_count;
+  uint4 list[kChunk];    // listed vectors of a chunk
+  int list_at[kChunk];   // and where they are
+  u64 buf[kBuffer];      // candidates
   u64 sel[kMaxK];
+  int hist[256];
+  int listed[3];         // of chunk c: entry c % 3, cleared while chunk c - 1 lists
+  int count, picked, digit, need, bin;
+  float warp_m[kThreads / 32], warp_s[kThreads / 32];
+  float m, s;            // this CTA's log-sum-exp parts
+  int out_count;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -183,20 +190,45 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Cut buf[0, n) to its `want` largest keys (all of them when n <= want): they end in
+__device__ __forceinline__ u64 pack2(float a, float b) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(u64 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Cut sc.buf[0, n) to its `want` largest keys (all of them when n <= want): they end in
 // sc.sel, in no order; returns how many.  Radix selection from the top digit, left as
-// soon as the digit's entries are exactly those still wanted.  All threads call it.
-__device__ __forceinline__ int select(const u64* buf, int n, int want, Scratch& sc) {
+// soon as a digit's entries are exactly those still wanted; digits in which all keys
+// agree (a 16-bit type's lower value bits, an index's leading ones) are left out.
+// All threads call it; they have passed a barrier since the last write to the buffer.
+template <int VALUE_BITS>
+__device__ __forceinline__ int select(int n, int want, int64_t v, Scratch& sc) {
   const int tid = threadIdx.x;
   if (tid == 0) sc.picked = 0;
   u64 prefix = 0, mask = 0;
   if (n > want) {
     int need = want;
     for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) sc.hist[i] = 0;
+      if (shift >= 32 ? shift < 64 - VALUE_BITS : (shift > 0 && v <= (int64_t(1) << shift))) continue;
+      sc.hist[tid] = 0;
       __syncthreads();
       for (int i = tid; i < n; i += kThreads) {
-        const u64 k = buf[i];
+        const u64 k = sc.buf[i];
         if ((k & mask) == prefix) atomicAdd(&sc.hist[(k >> shift) & 255], 1);
       }
       __syncthreads();
@@ -215,180 +247,319 @@ __device__ __forceinline__ int select(const u64* buf, int n, int want, Scratch& 
         }
         before -= sum;
         if (before < need && need <= before + sum) {
-          int j = 0;
-          while (before + own[j] < need) before += own[j++];
-          sc.digit = 255 - 8 * tid - j;
-          sc.need = need - before;
-          sc.count = own[j];  // scratch use; the caller sets it again
+          bool open = true;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (open && before + own[j] >= need) {
+              sc.digit = 255 - 8 * tid - j;
+              sc.need = need - before;
+              sc.bin = own[j];
+              open = false;
+            }
+            before += own[j];
+          }
         }
       }
       __syncthreads();
       prefix |= static_cast<u64>(sc.digit) << shift;
       mask |= 255ull << shift;
       need = sc.need;
-      const bool done = sc.count == need;
-      __syncthreads();
-      if (done) break;
+      if (sc.bin == need) break;
     }
-  } else {
-    __syncthreads();
   }
+  __syncthreads();
   for (int i = tid; i < n; i += kThreads) {
-    const u64 k = buf[i];
-    if (n <= want || (k & mask) >= prefix) sc.sel[atomicAdd(&sc.picked, 1)] = k;
+    const u64 k = sc.buf[i];
+    if ((k & mask) >= prefix) sc.sel[atomicAdd(&sc.picked, 1)] = k;
   }
   __syncthreads();
   return n < want ? n : want;
 }
 
-// The smallest key in sc.sel[0, n): what a later element has to pass.
-__device__ __forceinline__ u64 lowest(const Scratch& sc, int n) {
-  u64 low = ~0ull;
-  for (int i = threadIdx.x & 31; i < n; i += 32) low = sc.sel[i] < low ? sc.sel[i] : low;
-  for (int o = 16; o; o >>= 1) {
-    const u64 other = __shfl_xor_sync(0xffffffffu, low, o);
-    low = other < low ? other : low;
+// sc.buf[0, n) as runs of 32, each in falling order (the last filled up with zeros).
+// Run i is warp i % 8's.
+__device__ __forceinline__ void sort_runs(int n, Scratch& sc) {
+  const int lane = threadIdx.x & 31;
+  for (int at = (threadIdx.x & ~31); at < n; at += kThreads) {
+    u64 key = at + lane < n ? sc.buf[at + lane] : 0;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+      for (int o = size / 2; o; o /= 2) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, key, o);
+        const bool upper = (lane & o) != 0, falling = (lane & size) == 0;
+        key = (upper == falling) == (key > other) ? other : key;
+      }
+    }
+    sc.buf[at + lane] = key;
   }
-  return low;
+}
+
+// emit(key, number of keys above it) for every key of the sorted runs.
+template <typename F>
+__device__ __forceinline__ void rank_runs(int n, const Scratch& sc, F emit) {
+  const int lane = threadIdx.x & 31;
+  for (int at = (threadIdx.x & ~31); at < n; at += kThreads) {
+    const u64 key = sc.buf[at + lane];
+    int rank = lane;
+    for (int run = 0; run < n; run += 32) {
+      if (run == at) continue;
+      int above = 0;
+#pragma unroll
+      for (int o = 16; o; o /= 2) above += sc.buf[run + above + o - 1] > key ? o : 0;
+      rank += above + (sc.buf[run + above] > key ? 1 : 0);
+    }
+    if (at + lane < n) emit(key, rank);
+  }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch, int k,
-                                                       float scale, float inv_tau, void* __restrict__ values,
-                                                       int64_t* __restrict__ indices, float* __restrict__ lse) {
+__global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
+                                                          int k, float scale, float inv_tau, void* __restrict__ values,
+                                                          int64_t* __restrict__ indices, float* __restrict__ lse) {
   using K = Kind<T>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  Scratch& sc = *reinterpret_cast<Scratch*>(smem);
-  u64* buf = reinterpret_cast<u64*>(smem + ((sizeof(Scratch) + 15) & ~size_t(15)));
+  constexpr int kBits = 8 * sizeof(T);
+  __shared__ __align__(16) Scratch sc;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks());
   const int part = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t low16 = sizeof(T) == 4 ? 0xff800000u : (K::kBrain ? 0xff80ff80u : 0xfc00fc00u);
+  const uint4 nothing = make_uint4(low16, low16, low16, low16);  // -inf
+  uint4 cur[kVecs];
+
+  // [0, head) and [tail, v) are read one element at a time, the vectors between them
+  // are shared among the parts in runs of whole vectors.
   const int64_t row = blockIdx.x / parts;
   const T* x = logits + row * pitch;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  // [0, head) and [tail, v) are read one element at a time, the vectors between
-  // them are shared among the parts in runs of whole vectors.
-  int64_t head = static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T);
-  if (head > v) head = v;
-  const int64_t vecs = (v - head) / K::kPer;
-  const int64_t tail = head + vecs * K::kPer;
-  const int64_t w0 = vecs * part / parts, w1 = vecs * (part + 1) / parts;
-  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
-
-  if (tid == 0) sc.count = 0;
-  __syncthreads();
+  int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
+  if (head > v) head = static_cast<int>(v);
+  const int vecs = static_cast<int>((v - head) / K::kPer);
+  const int tail = head + vecs * K::kPer;
+  const int w0 = static_cast<int>(static_cast<int64_t>(vecs) * part / parts);
+  const int w1 = static_cast<int>(static_cast<int64_t>(vecs) * (part + 1) / parts);
+  // Stream j of this warp is vectors [(warp kVecs + j) rounds 32, + 32 rounds) of the part.
+  const int rounds = (w1 - w0 + kChunk - 1) / kChunk;
+  const uint4* xs = reinterpret_cast<const uint4*>(x + head) + w0 + (warp * kVecs * rounds) * 32 + lane;
+  const int left = w1 - w0 - (warp * kVecs * rounds) * 32 - lane;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) cur[j] = rounds && j * rounds * 32 < left ? __ldcs(xs + j * rounds * 32) : nothing;
+  if (tid == 0) sc.count = sc.listed[0] = sc.listed[1] = sc.listed[2] = 0;
   // scale = log2(e) / tau.  The reference m2 is the rounded product the exponents
   // use, so that log2(sum) + m2 carries no error from rounding it.
-  float m = -1e30f, m2 = fmaxf(-1e30f * scale, -3e38f), s = 0.0f;
+  float m = -1e30f, m2 = fmaxf(-1e30f * scale, -3e38f);
+  float s = 0.0f;
+  const u64 scale2 = pack2(scale, scale);
+  u64 s2 = 0;  // two running sums
   auto raise = [&](float to) {
     const float n2 = to * scale;
-    s *= exp2_fast(m2 - n2);
+    const float f = exp2_fast(m2 - n2);
+    const float2 both = unpack2(s2);
+    s *= f;
+    s2 = pack2(both.x * f, both.y * f);
     m = to;
     m2 = n2;
   };
-  uint32_t limit_key = 0;  // elements with a key above it (strictly) are candidates
+  u64 limit_key = 0;  // elements whose key is above it are candidates
   typename K::Limit limit = K::limit(__int_as_float(0x7fffffff));
-  auto offer = [&](uint32_t key, int64_t index) {
-    if (key > limit_key) {
-      const int at = atomicAdd(&sc.count, 1);
-      buf[at] = full_key(key, index);
-    }
-  };
+  // Vectors with an element above the value of `key`; NaN (all of them) for none.  A
+  // value between -0 and +0 does not exist: the one below stands in.
   auto set_limit = [&](uint32_t key) {
-    // The value just below `key + 1`; a key between -0 and +0 does not exist.
-    limit_key = key;
     uint32_t as = key;
-    if constexpr (sizeof(T) == 2) as = key & 0xffff0000u;
-    if (as == 0x7fffffffu || as == 0x7fff0000u) as -= sizeof(T) == 2 ? 0x10000u : 1u;
-    limit = K::limit(key == 0 ? __int_as_float(0x7fffffff) : value_of_key<T>(as));
+    if constexpr (kBits == 16) as = key & 0xffff0000u;
+    if (as == 0x7fffffffu || as == 0x7fff0000u) as -= kBits == 16 ? 0x10000u : 1u;
+    limit = K::limit(value_of_key<T>(as));
   };
-  auto add_vec = [&](const uint4& q) {
-    const float t = K::top(q);
-    if (t > m) raise(t);
-#pragma unroll
-    for (int i = 0; i < K::kPer; ++i) s += exp2_fast(fmaf(K::value(q, i), scale, -m2));
+  // Cut the buffer to k and raise the threshold to the k-th.
+  auto cut = [&](int n) {
+    const int kept = select<kBits>(n, k, v, sc);
+    u64 low = ~0ull;
+    for (int i = tid; i < kept; i += kThreads) sc.buf[i] = sc.sel[i];
+    for (int i = lane; i < kept; i += 32) low = sc.sel[i] < low ? sc.sel[i] : low;
+    for (int o = 16; o; o >>= 1) {
+      const u64 other = __shfl_xor_sync(0xffffffffu, low, o);
+      low = other < low ? other : low;
+    }
+    if (kept == k) limit_key = low;
+    if (tid == 0) sc.count = kept;
+    __syncthreads();
+    return kept;
   };
-  auto offer_vec = [&](const uint4& q, int64_t vec) {
-    if (K::above(q, limit)) {
-      const int64_t base = head + vec * K::kPer;
+  // The first threshold: the r-th largest of the threads' maxima over `cur`.
+  auto threshold = [&](bool any, int r) {
+    float best = K::top(cur[0]);
 #pragma unroll
-      for (int i = 0; i < K::kPer; ++i) offer(K::key(q, i), base + i);
+    for (int j = 1; j < kVecs; ++j) best = fmaxf(best, K::top(cur[j]));
+    if (!(best == best)) best = -INFINITY;
+    // The maximum of rank r - 1 among all.  A NaN only lowers the maximum seen here,
+    // which a bound may be; threads without an element come last.
+    sc.buf[tid] = (static_cast<u64>(any ? rising32(__float_as_uint(best)) : 0u) << 32) | static_cast<u64>(tid);
+    __syncwarp();
+    sort_runs(kThreads, sc);
+    __syncthreads();
+    rank_runs(kThreads, sc, [&](u64 key, int rank) {
+      if (rank == r - 1) sc.digit = static_cast<int>(key >> 32);
+    });
+    __syncthreads();
+    const uint32_t t = static_cast<uint32_t>(sc.digit);
+    limit_key = 0;
+    limit = K::limit(__int_as_float(0x7fffffff));
+    // As a value of the type, rounded down; candidates are at or above it.  (Below the
+    // key of -inf there is no value, and no bound.)
+    const float f = __uint_as_float(bits_of_rising32(t));
+    if (t && f == f) {
+      const uint32_t key = K::key_at_most(f);
+      limit_key = static_cast<u64>(key) << 32;
+      set_limit(key - 1);
     }
   };
-
-  // First vectors: the threads' maxima give the first threshold.
-  uint4 cur[kVecs], nxt[kVecs];
-  auto load = [&](uint4 (&q)[kVecs], int64_t chunk) {
-#pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      const int64_t w = w0 + (chunk * kVecs + j) * kThreads + tid;
-      if (w < w1) q[j] = __ldg(xv + w);
-    }
-  };
-  const int64_t chunks = (w1 - w0 + kThreads * kVecs - 1) / (kThreads * kVecs);
-  load(cur, 0);
-  {
-    uint32_t best = 0;
-#pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      if (w0 + j * kThreads + tid < w1) {
-#pragma unroll
-        for (int i = 0; i < K::kPer; ++i) best = max(best, K::key(cur[j], i));
-      }
-    }
-    // Largest t, in steps of 2^16, that k threads' maxima reach: bit by bit.
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t with = t | (1u << bit);
-      if (__syncthreads_count(best >= with) >= k) t = with;
-    }
-    if (t) set_limit(t - 1);
-  }
-  // The row's unaligned ends belong to the first part: the head before the vectors
-  // and the tail behind them, in index order, as the strict threshold asks.
-  auto one = [&](int64_t i) {
+  auto one = [&](int i) {  // an element of the row's unaligned ends
     const uint32_t key = K::scalar_key(x + i);
     const float f = value_of_key<T>(key);
     if (f > m) raise(f);
     s += exp2_fast(fmaf(f, scale, -m2));
-    offer(key, i);
+    if (full_key(key, i) > limit_key) sc.buf[atomicAdd(&sc.count, 1)] = full_key(key, i);
   };
-  if (part == 0 && tid < head) one(tid);
-  for (int64_t c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) load(nxt, c + 1);
-    bool many = false;
+  auto round_top = [&]() {
+    float tops = K::top(cur[0]);
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      const int64_t w = (c * kVecs + j) * kThreads + tid;
-      if (w0 + w < w1) {
-        add_vec(cur[j]);
-        offer_vec(cur[j], w0 + w);
-      }
-    }
-    // A thread that finds the count above kKeep after its own entries: the last to
-    // add one does, so the vote is the same as reading the final count.
-    many = *reinterpret_cast<volatile int*>(&sc.count) > kKeep;
-    if (__syncthreads_or(many)) {
-      const int n = sc.count;
-      __syncthreads();
-      const int kept = select(buf, n, k, sc);
-      for (int i = tid; i < kept; i += kThreads) buf[i] = sc.sel[i];
-      if (kept == k) {
-        const u64 low = lowest(sc, kept);
-        set_limit(static_cast<uint32_t>(low >> 32));
-      }
-      __syncthreads();
-      if (tid == 0) sc.count = kept;
-      __syncthreads();
-    }
+    for (int j = 1; j < kVecs; ++j) tops = fmaxf(tops, K::top(cur[j]));
+    if (tops > m) raise(tops);
+  };
+  auto add = [&](const uint4& q, u64 minus) {
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) cur[j] = nxt[j];
+    for (int i = 0; i < K::kPer; i += 2) {
+      const float2 z = K::pair_value(q, i / 2);
+      const float2 e = unpack2(fma2(pack2(z.x, z.y), scale2, minus));
+      s2 = add2(s2, pack2(exp2_fast(e.x), exp2_fast(e.y)));
+    }
+  };
+  // Listed vectors' elements that pass to the buffer, in batches that it has room for.
+  // All threads call it, behind a barrier; ends with one.
+  auto work_off = [&](int listed) {
+    int done = 0, count = sc.count;
+    __syncthreads();
+    while (done < listed) {
+      const int batch = min(listed - done, kBuffer - count);
+      for (int i = done + tid; i < done + batch; i += kThreads) {
+        const u64 key = full_key(K::stored_key(&sc.list[i / K::kPer], i % K::kPer), sc.list_at[i / K::kPer] + i % K::kPer);
+        if (key > limit_key) sc.buf[atomicAdd(&sc.count, 1)] = key;
+      }
+      done += batch;
+      __syncthreads();
+      count = sc.count;
+      __syncthreads();
+      if (count >= kBuffer / 2) count = cut(count);
+    }
+    return count;
+  };
+  const bool ends = part == 0;
+  bool safe = true;
+  {
+    // The guess (its first round is loaded already).
+    const float share = rounds > 1 ? static_cast<float>(k) / rounds : static_cast<float>(k);
+    const int r = min(k, static_cast<int>(share + 2.5f * sqrtf(share)) + 3);
+    threshold(left > 0, r);
+    if (ends && tid < head) one(tid);
+    // Every stream of the thread full (all but the part's last ones): no bounds to look at.
+    auto stream = [&](auto whole) {
+      constexpr bool full = decltype(whole)::value;
+      const uint4* at = xs;
+      int64_t index = head + (w0 + (warp * kVecs * rounds) * 32 + lane) * static_cast<int64_t>(K::kPer);
+      for (int c = 0; c < rounds; ++c) {
+        round_top();
+        const u64 minus = pack2(-m2, -m2);
+        at += 32;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+          const uint4 q = cur[j];
+          if (full) {
+            if (c + 1 < rounds) cur[j] = __ldcs(at + j * rounds * 32);
+          } else {
+            const int w = (j * rounds + c + 1) * 32;
+            cur[j] = c + 1 < rounds && w < left ? __ldcs(xs + w) : nothing;
+          }
+          if (K::above(q, limit) && (full || (j * rounds + c) * 32 < left)) {
+            const int slot = atomicAdd(&sc.listed[0], 1);
+            if (slot < kChunk) {
+              sc.list[slot] = q;
+              sc.list_at[slot] = static_cast<int>(index) + (j * rounds + c) * 32 * K::kPer;
+            } else {
+              c = rounds;  // overflow: the other form will do it
+            }
+          }
+          add(q, minus);
+        }
+      }
+    };
+    if (__all_sync(0xffffffffu, ((kVecs - 1) * rounds + rounds - 1) * 32 < left)) {
+      stream(std::true_type{});
+    } else {
+      stream(std::false_type{});
+    }
+    __syncthreads();
+    const int listed = sc.listed[0];
+    if (listed <= kChunk) {
+      const int count = work_off(listed * K::kPer);
+      // (The tail's elements are still to come, the guess counts without them.)
+      safe = count < k && limit_key != 0;
+    }
   }
-
-  if (part == 0 && tid < v - tail) one(tail + tid);
+  if (safe) {
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head) + w0 + tid;
+    const int own = w1 - w0 - tid;  // vectors from this thread's first on
+    __syncthreads();
+    if (tid == 0) sc.count = sc.listed[0] = sc.listed[1] = sc.listed[2] = 0;
+    m = -1e30f;
+    m2 = fmaxf(-1e30f * scale, -3e38f);
+    s = 0.0f;
+    s2 = 0;
+    auto load = [&](int first) {
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) {
+        const int w = first + j * kThreads;
+        cur[j] = w < own ? __ldg(xv + w) : nothing;
+      }
+    };
+    load(0);
+    threshold(own > 0, k);
+    // The head before the vectors and the tail behind them: in index order, as the
+    // strict threshold asks.
+    if (ends && tid < head) one(tid);
+    int turn = 0;
+    for (int first = 0; first < w1 - w0; first += kChunk) {
+      const int next_turn = turn == 2 ? 0 : turn + 1;
+      if (tid == 0) sc.listed[next_turn] = 0;  // read last before the previous barrier
+      round_top();
+      const u64 minus = pack2(-m2, -m2);
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) {
+        if (K::above(cur[j], limit) && first + j * kThreads < own) {
+          const int at = atomicAdd(&sc.listed[turn], 1);
+          sc.list[at] = cur[j];
+          sc.list_at[at] = head + (w0 + tid + first + j * kThreads) * K::kPer;
+        }
+        add(cur[j], minus);
+      }
+      load(first + kChunk);
+      __syncthreads();
+      const int listed = sc.listed[turn] * K::kPer;
+      turn = next_turn;
+      if (listed) {
+        const int count = work_off(listed);
+        if (count >= 2 * k) cut(count);
+        // Strictly: later vectors have higher indices.
+        if (limit_key & 0xffffffffull) set_limit(static_cast<uint32_t>(limit_key >> 32));
+      }
+    }
+  }
+  if (ends && tid < v - tail) one(tail + tid);
 
   // Log-sum-exp of this CTA.
+  {
+    const float2 both = unpack2(s2);
+    s += both.x + both.y;
+  }
   for (int o = 16; o; o >>= 1) {
     const float om = __shfl_xor_sync(0xffffffffu, m2, o), os = __shfl_xor_sync(0xffffffffu, s, o);
     const float big = fmaxf(m2, om);
@@ -400,9 +571,16 @@ __global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ log
     sc.warp_s[warp] = s;
   }
   __syncthreads();
-  const int n = sc.count;
+  // This CTA's k largest in falling order.
+  int n = sc.count;
   __syncthreads();
-  int kept = select(buf, n, k, sc);
+  if (n > kRankable) n = cut(n);
+  sort_runs(n, sc);
+  __syncthreads();
+  const int kept = n < k ? n : k;
+  rank_runs(n, sc, [&](u64 key, int rank) {
+    if (rank < kept) sc.sel[rank] = key;
+  });
   if (tid == 0) {
     float big = sc.warp_m[0];
     for (int w = 1; w < kThreads / 32; ++w) big = fmaxf(big, sc.warp_m[w]);
@@ -414,71 +592,63 @@ __global__ void __launch_bounds__(kThreads) top_kernel(const T* __restrict__ log
   }
   if (parts > 1) {
     cluster.sync();
-    if (part == 0) {
-      // Gather the other parts' selections behind this one's.
-      for (int i = tid; i < kept; i += kThreads) buf[i] = sc.sel[i];
-      int at = kept;
-      for (int c = 1; c < parts; ++c) {
-        const Scratch* other = cluster.map_shared_rank(&sc, c);
-        const int theirs = other->out_count;
-        for (int i = tid; i < theirs; i += kThreads) buf[at + i] = other->sel[i];
-        at += theirs;
-      }
-      if (tid == 0) {
-        float big = sc.m;
-        for (int c = 1; c < parts; ++c) big = fmaxf(big, cluster.map_shared_rank(&sc, c)->m);
-        float sum = 0.0f;
-        for (int c = 0; c < parts; ++c) {
-          const Scratch* other = cluster.map_shared_rank(&sc, c);
-          sum += other->s * exp2_fast(other->m - big);
-        }
-        sc.m = big;
-        sc.s = sum;
-      }
-      __syncthreads();
-      kept = select(buf, at, k, sc);
-    }
-    cluster.sync();
-    if (part != 0) return;
   } else {
     __syncthreads();
   }
-  // Rank of each selected key among them: its place in the output.
+  // An entry's place in the output: its place here and the entries above it in the
+  // other parts' lists.
   for (int i = tid; i < kept; i += kThreads) {
     const u64 key = sc.sel[i];
-    int rank = 0;
-    for (int j = 0; j < kept; ++j) rank += sc.sel[j] > key ? 1 : 0;
-    const uint32_t high = static_cast<uint32_t>(key >> 32);
-    K::store(values, row * k + rank, high);
-    indices[row * k + rank] = static_cast<int64_t>(0xffffffffull - (key & 0xffffffffull));
-    if (rank == 0) {
-      // The largest logit decides the cases that the sum cannot: NaN and infinities
-      // as they are, and logits beyond 1e30 (a row of the type's lowest value), where
-      // the logarithm of the count is below the logit's rounding.
-      const float topv = value_of_key<T>(high);
-      const float sum = sc.s;
-      lse[row] = (isnan(topv) || isinf(topv)) ? topv
-                 : sum > 0.0f && !isinf(sc.m)     ? (sc.m + log2f(sum)) * 0.6931471805599453f
-                                                   : topv * inv_tau;
+    int rank = i;
+    for (int c = 0; c < parts; ++c) {
+      if (c == part) continue;
+      const Scratch* other = cluster.map_shared_rank(&sc, c);
+      int lo = 0, hi = min(other->out_count, k - rank);  // (more than k - rank puts it out anyway)
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (other->sel[mid] > key) lo = mid + 1; else hi = mid;
+      }
+      rank += lo;
+      if (rank >= k) break;
+    }
+    if (rank < k) {
+      K::store(values, row * k + rank, static_cast<uint32_t>(key >> 32));
+      indices[row * k + rank] = static_cast<int64_t>(0xffffffffull - (key & 0xffffffffull));
     }
   }
+  if (part == 0 && tid == 0) {
+    u64 top = kept ? sc.sel[0] : 0;
+    float big = sc.m, sum = sc.s;
+    for (int c = 1; c < parts; ++c) {
+      const Scratch* other = cluster.map_shared_rank(&sc, c);
+      const u64 t = other->out_count ? other->sel[0] : 0;
+      top = t > top ? t : top;
+      const float om = other->m, to = fmaxf(big, om);
+      sum = sum * exp2_fast(big - to) + other->s * exp2_fast(om - to);
+      big = to;
+    }
+    // The largest logit decides the cases that the sum cannot: NaN and infinities as
+    // they are, and logits beyond 1e30 (a row of the type's lowest value), where the
+    // logarithm of the count is below the logit's rounding.
+    const float topv = value_of_key<T>(static_cast<uint32_t>(top >> 32));
+    lse[row] = (isnan(topv) || isinf(topv)) ? topv
+               : sum > 0.0f && !isinf(big)     ? (big + log2f(sum)) * 0.6931471805599453f
+                                                : topv * inv_tau;
+  }
+  if (parts > 1) cluster.sync();  // the others' lists stay until all have read them
 }
 
 template <typename T>
 int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, float temperature, void* values,
            int64_t* indices, float* lse, cudaStream_t st) {
-  auto kern = top_kernel<T>;
-  const int smem = static_cast<int>(((sizeof(Scratch) + 15) & ~size_t(15)) + capacity<T>() * sizeof(u64));
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(SB_ECUDA, std::string("top_kernel attributes: ") + cudaGetErrorString(e));
-  // Few rows are split over a cluster while the parts keep a chunk of work each.
+  // Few rows are split over a cluster (at most the portable eight CTAs) while the parts
+  // keep half a chunk each.
   int parts = 1;
   const int sms = device_sm_count();
-  while (parts < 8 && rows * parts * 2 <= 2 * sms && v / (parts * 2) >= chunk_elems<T>() / 2) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= 4 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -486,8 +656,8 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(logits), v, pitch, k, 1.4426950408889634f / temperature,
-                         1.0f / temperature, values, indices, lse);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, top_kernel<T>, static_cast<const T*>(logits), v, pitch, k,
+                                           1.4426950408889634f / temperature, 1.0f / temperature, values, indices, lse);
   if (e != cudaSuccess) return fail(SB_ECUDA, std::string("top_kernel: ") + cudaGetErrorString(e));
   count_launch();
   return check_launch("top_kernel");

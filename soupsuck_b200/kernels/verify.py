@@ -16,6 +16,12 @@ import torch
 from .. import _lib
 from .._spec import LONG, SINGLE, WIDE_FLOATS, Operand, admit, refuse
 
+_PROBS = Operand(*WIDE_FLOATS, ndim=3, layout=None)
+_LIKE = {dtype: Operand(dtype, ndim=3, layout=None, optional=True) for dtype in WIDE_FLOATS}
+_TOKENS = Operand(LONG, ndim=2, layout=None)
+_NUMBERS = Operand(SINGLE, ndim=2, layout=None)
+_LENS = Operand(LONG, ndim=1, layout=None, optional=True)
+
 
 def _rows_unit(entry, name, t):
     if t.shape[-1] > 1 and t.stride(-1) != 1:
@@ -32,12 +38,9 @@ def verify_drafts(target_probs, draft_tokens, uniforms, noise, draft_probs=None,
     rejected."""
     entry = "verify_drafts"
     device = target_probs.device if isinstance(target_probs, torch.Tensor) else None
-    admit(entry, device, target_probs=(target_probs, Operand(*WIDE_FLOATS, ndim=3, layout=None)))
-    admit(entry, device, draft_tokens=(draft_tokens, Operand(LONG, ndim=2, layout=None)),
-          uniforms=(uniforms, Operand(SINGLE, ndim=2, layout=None)),
-          noise=(noise, Operand(SINGLE, ndim=2, layout=None)),
-          draft_probs=(draft_probs, Operand(target_probs.dtype, ndim=3, layout=None, optional=True)),
-          draft_lens=(draft_lens, Operand(LONG, ndim=1, layout=None, optional=True)))
+    admit(entry, device, target_probs=(target_probs, _PROBS))
+    admit(entry, device, draft_tokens=(draft_tokens, _TOKENS), uniforms=(uniforms, _NUMBERS), noise=(noise, _NUMBERS),
+          draft_probs=(draft_probs, _LIKE[target_probs.dtype]), draft_lens=(draft_lens, _LENS))
     batch, places, vocab = target_probs.shape
     drafts = draft_tokens.shape[1]
     lines_up = (places == drafts + 1 and draft_tokens.shape[0] == batch
@@ -55,7 +58,7 @@ def verify_drafts(target_probs, draft_tokens, uniforms, noise, draft_probs=None,
     _rows_unit(entry, "noise", noise)
     if draft_probs is not None:
         _rows_unit(entry, "draft_probs", draft_probs)
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         tokens_in, u = draft_tokens.contiguous(), uniforms.contiguous()
         lens = None if draft_lens is None else draft_lens.contiguous()
         accepted = torch.empty(batch, device=device, dtype=LONG)
@@ -66,5 +69,5 @@ def verify_drafts(target_probs, draft_tokens, uniforms, noise, draft_probs=None,
                       _lib.ptr(q), 0 if q is None else q.stride(0), 0 if q is None else q.stride(1),
                       _lib.wide_dtype_code(target_probs.dtype), batch, drafts, vocab, tokens_in.data_ptr(),
                       u.data_ptr(), noise.data_ptr(), noise.stride(0), _lib.ptr(lens), accepted.data_ptr(),
-                      tokens.data_ptr(), _lib.stream_of(device))
+                      tokens.data_ptr(), _lib.raw_stream(device))
     return accepted, tokens
