@@ -37,10 +37,12 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256;
 constexpr int kMaxK = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kVecs = 4;                      // 16-byte vectors per thread and chunk
 constexpr int kChunk = kThreads * kVecs;      // vectors
 constexpr int kBuffer = 2048;
 constexpr int kRankable = 512;                // candidates that are sorted without a selection
+constexpr int kMaxParts = 8;                  // CTAs of a row (the portable cluster limit)
 constexpr int kPerSm = 4;
 
 using u64 = unsigned long long;
@@ -181,7 +183,6 @@ struct Scratch {
   int count, picked, digit, need, bin;
   float warp_m[kThreads / 32], warp_s[kThreads / 32];
   float m, s;            // this CTA's log-sum-exp parts
-  int out_count;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -338,12 +339,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   const int tail = head + vecs * K::kPer;
   const int w0 = static_cast<int>(static_cast<int64_t>(vecs) * part / parts);
   const int w1 = static_cast<int>(static_cast<int64_t>(vecs) * (part + 1) / parts);
-  // Stream j of this warp is vectors [(warp kVecs + j) rounds 32, + 32 rounds) of the part.
+  // Stream j of this warp is vectors [(j kWarps + warp) rounds 32, + 32 rounds) of the part.
   const int rounds = (w1 - w0 + kChunk - 1) / kChunk;
-  const uint4* xs = reinterpret_cast<const uint4*>(x + head) + w0 + (warp * kVecs * rounds) * 32 + lane;
-  const int left = w1 - w0 - (warp * kVecs * rounds) * 32 - lane;
+  const uint4* xs = reinterpret_cast<const uint4*>(x + head) + w0 + (warp * rounds) * 32 + lane;
+  const int left = w1 - w0 - (warp * rounds) * 32 - lane;
 #pragma unroll
-  for (int j = 0; j < kVecs; ++j) cur[j] = rounds && j * rounds * 32 < left ? __ldcs(xs + j * rounds * 32) : nothing;
+  for (int j = 0; j < kVecs; ++j) cur[j] = rounds && j * kWarps * rounds * 32 < left ? __ldcs(xs + j * kWarps * rounds * 32) : nothing;
   if (tid == 0) sc.count = sc.listed[0] = sc.listed[1] = sc.listed[2] = 0;
   // scale = log2(e) / tau.  The reference m2 is the rounded product the exponents
   // use, so that log2(sum) + m2 carries no error from rounding it.
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     auto stream = [&](auto whole) {
       constexpr bool full = decltype(whole)::value;
       const uint4* at = xs;
-      int64_t index = head + (w0 + (warp * kVecs * rounds) * 32 + lane) * static_cast<int64_t>(K::kPer);
+      int64_t index = head + (w0 + (warp * rounds) * 32 + lane) * static_cast<int64_t>(K::kPer);
       for (int c = 0; c < rounds; ++c) {
         round_top();
         const u64 minus = pack2(-m2, -m2);
@@ -474,16 +475,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
         for (int j = 0; j < kVecs; ++j) {
           const uint4 q = cur[j];
           if (full) {
-            if (c + 1 < rounds) cur[j] = __ldcs(at + j * rounds * 32);
+            if (c + 1 < rounds) cur[j] = __ldcs(at + j * kWarps * rounds * 32);
           } else {
-            const int w = (j * rounds + c + 1) * 32;
+            const int w = (j * kWarps * rounds + c + 1) * 32;
             cur[j] = c + 1 < rounds && w < left ? __ldcs(xs + w) : nothing;
           }
-          if (K::above(q, limit) && (full || (j * rounds + c) * 32 < left)) {
+          if (K::above(q, limit) && (full || (j * kWarps * rounds + c) * 32 < left)) {
             const int slot = atomicAdd(&sc.listed[0], 1);
             if (slot < kChunk) {
               sc.list[slot] = q;
-              sc.list_at[slot] = static_cast<int>(index) + (j * rounds + c) * 32 * K::kPer;
+              sc.list_at[slot] = static_cast<int>(index) + (j * kWarps * rounds + c) * 32 * K::kPer;
             } else {
               c = rounds;  // overflow: the other form will do it
             }
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
         }
       }
     };
-    if (__all_sync(0xffffffffu, ((kVecs - 1) * rounds + rounds - 1) * 32 < left)) {
+    if (__all_sync(0xffffffffu, ((kVecs - 1) * kWarps * rounds + rounds - 1) * 32 < left)) {
       stream(std::true_type{});
     } else {
       stream(std::false_type{});
@@ -581,6 +582,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   rank_runs(n, sc, [&](u64 key, int rank) {
     if (rank < kept) sc.sel[rank] = key;
   });
+  for (int i = kept + tid; i < kMaxK; i += kThreads) sc.sel[i] = 0;
   if (tid == 0) {
     float big = sc.warp_m[0];
     for (int w = 1; w < kThreads / 32; ++w) big = fmaxf(big, sc.warp_m[w]);
@@ -588,7 +590,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     for (int w = 0; w < kThreads / 32; ++w) sum += sc.warp_s[w] * exp2_fast(sc.warp_m[w] - big);
     sc.m = big;
     sc.s = sum;
-    sc.out_count = kept;
   }
   if (parts > 1) {
     cluster.sync();
@@ -596,44 +597,52 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     __syncthreads();
   }
   // An entry's place in the output: its place here and the entries above it in the
-  // other parts' lists.
+  // other parts' lists, searched side by side (a remote load takes about as long as
+  // eight at once).
   for (int i = tid; i < kept; i += kThreads) {
     const u64 key = sc.sel[i];
     int rank = i;
-    for (int c = 0; c < parts; ++c) {
-      if (c == part) continue;
-      const Scratch* other = cluster.map_shared_rank(&sc, c);
-      int lo = 0, hi = min(other->out_count, k - rank);  // (more than k - rank puts it out anyway)
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (other->sel[mid] > key) lo = mid + 1; else hi = mid;
+    if (parts > 1) {
+      int above[kMaxParts] = {};
+      for (int o = 1 << (31 - __clz(k)); o; o >>= 1) {
+        u64 at[kMaxParts];
+#pragma unroll
+        for (int c = 0; c < kMaxParts; ++c) {
+          if (c < parts && above[c] + o <= k) at[c] = cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1];
+        }
+#pragma unroll
+        for (int c = 0; c < kMaxParts; ++c) above[c] += c < parts && above[c] + o <= k && at[c] > key ? o : 0;
       }
-      rank += lo;
-      if (rank >= k) break;
+      rank = 0;
+#pragma unroll
+      for (int c = 0; c < kMaxParts; ++c) rank += above[c];
     }
     if (rank < k) {
       K::store(values, row * k + rank, static_cast<uint32_t>(key >> 32));
       indices[row * k + rank] = static_cast<int64_t>(0xffffffffull - (key & 0xffffffffull));
     }
   }
-  if (part == 0 && tid == 0) {
-    u64 top = kept ? sc.sel[0] : 0;
-    float big = sc.m, sum = sc.s;
-    for (int c = 1; c < parts; ++c) {
-      const Scratch* other = cluster.map_shared_rank(&sc, c);
-      const u64 t = other->out_count ? other->sel[0] : 0;
+  if (part == 0 && warp == 0) {
+    const Scratch* from = lane < parts ? cluster.map_shared_rank(&sc, lane) : &sc;
+    u64 top = from->sel[0];
+    float big = from->m, sum = lane < parts ? from->s : 0.0f;
+    for (int o = kMaxParts / 2; o; o >>= 1) {
+      const u64 t = __shfl_xor_sync(0xffffffffu, top, o);
       top = t > top ? t : top;
-      const float om = other->m, to = fmaxf(big, om);
-      sum = sum * exp2_fast(big - to) + other->s * exp2_fast(om - to);
+      const float om = __shfl_xor_sync(0xffffffffu, big, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float to = fmaxf(big, om);
+      sum = sum * exp2_fast(big - to) + os * exp2_fast(om - to);
       big = to;
     }
     // The largest logit decides the cases that the sum cannot: NaN and infinities as
     // they are, and logits beyond 1e30 (a row of the type's lowest value), where the
     // logarithm of the count is below the logit's rounding.
     const float topv = value_of_key<T>(static_cast<uint32_t>(top >> 32));
-    lse[row] = (isnan(topv) || isinf(topv)) ? topv
-               : sum > 0.0f && !isinf(big)     ? (big + log2f(sum)) * 0.6931471805599453f
-                                                : topv * inv_tau;
+    if (lane == 0) {
+      lse[row] = (isnan(topv) || isinf(topv)) ? topv
+                 : sum > 0.0f && !isinf(big)     ? (big + log2f(sum)) * 0.6931471805599453f
+                                                  : topv * inv_tau;
+    }
   }
   if (parts > 1) cluster.sync();  // the others' lists stay until all have read them
 }
@@ -645,7 +654,7 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   // keep half a chunk each.
   int parts = 1;
   const int sms = device_sm_count();
-  while (parts < 8 && rows * parts * 2 <= 4 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
+  while (parts < kMaxParts && rows * parts * 2 <= 4 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);

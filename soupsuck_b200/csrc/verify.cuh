@@ -29,8 +29,6 @@ template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; 
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-constexpr int kThreads = 512;
-
 struct Args {
   const void* target;
   const void* draft;
@@ -51,53 +49,131 @@ __device__ __forceinline__ unsigned long long pack(float score, int64_t v) {
          (0xffffffffull - static_cast<unsigned long long>(v));
 }
 
-template <typename T>
-__device__ __forceinline__ void race(float p, float q, float e, int64_t v, float& best, int64_t& at) {
-  const float r = __fsub_rn(p, q);
-  if (r > 0.0f) {
-    const float s = __fdiv_rn(r, e);
-    if (s > best) {
-      best = s;
-      at = v;
+// A thread's best so far.  `bar` is a little below it: r / e can only beat the best where
+// r > bar e, so the division is left to the few elements that pass (in fp32 rounding;
+// bests below 1e-30 keep no bar).
+struct Best {
+  float score = 0.0f, bar = 0.0f;
+  int at = 0;
+  __device__ __forceinline__ void race(float p, float q, float e, int v) {
+    const float r = __fsub_rn(p, q);
+    // (-1e-44: a product among the denormals may be rounded up by a whole one.)
+    if (r > fmaf(bar, e, -1e-44f) && r > 0.0f) {
+      const float s = __fdiv_rn(r, e);
+      if (s > score) {
+        score = s;
+        bar = s < 1e-30f ? 0.0f : s * 0.999999f;
+        at = v;
+      }
     }
   }
-}
+};
 
-// One CTA's share [v0, v1) of the row: elements v0 + tid, v0 + tid + kThreads, ...
-template <typename T>
-__device__ void scan(const T* p, const T* q, int64_t hot, const float* e, int64_t v0, int64_t v1, float& best,
-                     int64_t& at) {
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int kPer = 4;
+  static __device__ __forceinline__ float get(const uint4& q, int i) {
+    return __uint_as_float(i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w);
+  }
+};
+template <typename T> struct Vec16 {
+  static constexpr int kPer = 8;
+  static __device__ __forceinline__ float get(const uint4& q, int i) {
+    const uint32_t w = i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w;
+    const unsigned short b = static_cast<unsigned short>((i & 1) ? w >> 16 : w & 0xffffu);
+    return to_f32<T>(*reinterpret_cast<const T*>(&b));
+  }
+};
+template <> struct Vec<__half> : Vec16<__half> {};
+template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
+
+// One CTA's share [v0, v1) of the row.  16-byte loads where the three rows reach a
+// 16-byte boundary at the same element, single elements elsewhere (rows of an odd
+// vocabulary differ).  256 sequences x 5 drafts of 151936 fp32, 71 us at the copy rate:
+// 73.5 us in vectors, two in flight per row and thread so that four CTAs fit an SM
+// (four in flight, two CTAs: 114); of 151935 in single elements 87; with a division for
+// every element 155.
+template <typename T, bool DRAFT, int THREADS>
+__device__ __forceinline__ void scan(const T* p, const T* q, int hot, const float* e, int v0, int v1, Best& best) {
+  using V = Vec<T>;
+  constexpr int kPer = V::kPer;
+  auto single = [&](int v) { best.race(v == hot ? 0.0f : to_f32<T>(p[v]), DRAFT ? to_f32<T>(q[v]) : 0.0f, e[v], v); };
+  auto off = [](const void* x, int size, int mod) { return static_cast<int>(reinterpret_cast<uintptr_t>(x) / size % mod); };
+  const int at_p = off(p + v0, sizeof(T), kPer);
+  int tid = threadIdx.x;
+  if ((!DRAFT || off(q + v0, sizeof(T), kPer) == at_p) && off(e + v0, 4, 4) == at_p % 4) {
+    const int head = min((kPer - at_p) % kPer, v1 - v0);
+    const int vecs = (v1 - v0 - head) / kPer;
+    const int base = v0 + head;
+    if (tid < head) single(v0 + tid);
+    constexpr int kUnroll = 2;
+    constexpr int kE = kPer / 4;
+    const uint4* pv = reinterpret_cast<const uint4*>(p + base);
+    const uint4* qv = reinterpret_cast<const uint4*>(q + base);
+    const uint4* ev = reinterpret_cast<const uint4*>(e + base);
+    auto eat = [&](const uint4& a, const uint4& b, const uint4 (&c)[kE], int w) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int v = base + w * kPer + i;
+        best.race(!DRAFT && v == hot ? 0.0f : V::get(a, i), DRAFT ? V::get(b, i) : 0.0f, Vec<float>::get(c[i / 4], i % 4), v);
+      }
+    };
+    int w = tid;
+    for (; w + (kUnroll - 1) * THREADS < vecs; w += kUnroll * THREADS) {
+      uint4 a[kUnroll], b[kUnroll], c[kUnroll][kE];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        a[u] = __ldcs(pv + w + u * THREADS);
+        if (DRAFT) b[u] = __ldcs(qv + w + u * THREADS);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) c[u][i] = __ldcs(ev + (w + u * THREADS) * kE + i);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) eat(a[u], b[u], c[u], w + u * THREADS);
+    }
+    for (; w < vecs; w += THREADS) {
+      uint4 b = make_uint4(0, 0, 0, 0), c[kE];
+      const uint4 a = __ldcs(pv + w);
+      if (DRAFT) b = __ldcs(qv + w);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) c[i] = __ldcs(ev + w * kE + i);
+      eat(a, b, c, w);
+    }
+    const int v = base + vecs * kPer + tid;
+    if (v < v1) single(v);
+    return;
+  }
   constexpr int kUnroll = 8;
-  int64_t v = v0 + threadIdx.x;
-  for (; v + (kUnroll - 1) * kThreads < v1; v += kUnroll * kThreads) {
+  int v = v0 + tid;
+  for (; v + (kUnroll - 1) * THREADS < v1; v += kUnroll * THREADS) {
     float pv[kUnroll], qv[kUnroll], ev[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int64_t x = v + i * kThreads;
+      const int x = v + i * THREADS;
       pv[i] = to_f32<T>(p[x]);
-      qv[i] = q ? to_f32<T>(q[x]) : 0.0f;
+      qv[i] = DRAFT ? to_f32<T>(q[x]) : 0.0f;
       ev[i] = e[x];
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int64_t x = v + i * kThreads;
-      race<T>(x == hot ? 0.0f : pv[i], qv[i], ev[i], x, best, at);
+      const int x = v + i * THREADS;
+      best.race(!DRAFT && x == hot ? 0.0f : pv[i], qv[i], ev[i], x);
     }
   }
-  for (; v < v1; v += kThreads) race<T>(v == hot ? 0.0f : to_f32<T>(p[v]), q ? to_f32<T>(q[v]) : 0.0f, e[v], v, best, at);
+  for (; v < v1; v += THREADS) single(v);
 }
 
 // A cluster of CTAs per sequence: each repeats the short acceptance test, scans its
 // share of the vocabulary, and the best keys meet in distributed shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const Args a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks());
   const int part = static_cast<int>(cluster.block_rank());
   const int64_t b = blockIdx.x / parts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int s_accepted, s_len;
-  __shared__ unsigned long long s_warp[kThreads / 32];
+  __shared__ unsigned long long s_warp[THREADS / 32];
   __shared__ unsigned long long s_best;
   const T* target = static_cast<const T*>(a.target) + b * a.t_b;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + b * a.d_b : nullptr;
@@ -137,33 +213,45 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
   const bool rejected = n < s_len;
   const T* p = target + n * a.t_s;
   const T* q = rejected && draft ? draft + n * a.d_s : nullptr;
-  int64_t hot = rejected && !draft ? tokens[n] : -1;
+  int hot = -1;
+  if (rejected && !draft && tokens[n] >= 0 && tokens[n] < a.v) hot = static_cast<int>(tokens[n]);
   const float* e = a.noise + b * a.n_b;
-  const int64_t share = (a.v + parts - 1) / parts;
-  const int64_t v0 = part * share, v1 = v0 + share < a.v ? v0 + share : a.v;
+  // Shares of whole vectors of every type, in order.
+  const int64_t share = ((a.v + parts - 1) / parts + 7) / 8 * 8;
+  const int v0 = static_cast<int>(part * share < a.v ? part * share : a.v);
+  const int v1 = static_cast<int>(v0 + share < a.v ? v0 + share : a.v);
   unsigned long long key = 0;
   // The second round only where the residual is zero everywhere: p itself then.
   for (int round = 0; round < 2; ++round) {
-    float best = 0.0f;
-    int64_t at = 0;
-    scan<T>(p, q, hot, e, v0, v1, best, at);
-    key = best > 0.0f ? pack(best, at) : 0;
+    Best best;
+    if (q) {
+      scan<T, true, THREADS>(p, q, -1, e, v0, v1, best);
+    } else {
+      scan<T, false, THREADS>(p, p, hot, e, v0, v1, best);
+    }
+    key = best.score > 0.0f ? pack(best.score, best.at) : 0;
     for (int o = 16; o; o >>= 1) {
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
       key = other > key ? other : key;
     }
     if (lane == 0) s_warp[warp] = key;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < kThreads / 32; ++w) key = s_warp[w] > key ? s_warp[w] : key;
-      s_best = key;
+    if (warp == 0) {
+      key = lane < THREADS / 32 ? s_warp[lane] : 0;
+      for (int o = 16; o; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+        key = other > key ? other : key;
+      }
+      if (lane == 0) s_best = key;
     }
     cluster.sync();
-    key = 0;
-    for (int c = 0; c < parts; ++c) {
-      const unsigned long long other = *cluster.map_shared_rank(&s_best, c);
+    // Lane c takes part c's best (remote loads: all at once).
+    key = lane < parts ? *cluster.map_shared_rank(&s_best, lane) : 0;
+    for (int o = 4; o; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
       key = other > key ? other : key;
     }
+    key = __shfl_sync(0xffffffffu, key, 0);
     cluster.sync();
     if (key || !rejected) break;
     q = nullptr;
@@ -171,19 +259,19 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const Args a) {
   }
   if (part == 0) {
     int64_t* out = a.out + b * (a.drafts + 1);
-    for (int s = threadIdx.x; s <= a.drafts; s += kThreads) {
+    for (int s = threadIdx.x; s <= a.drafts; s += THREADS) {
       out[s] = s < n ? tokens[s] : (s == n && key ? static_cast<int64_t>(0xffffffffull - (key & 0xffffffffull)) : -1);
     }
     if (threadIdx.x == 0) a.accepted[b] = n;
   }
 }
 
-template <typename T>
+template <typename T, int THREADS>
 int launch(const Args& a, int64_t batch, int parts, cudaStream_t st) {
-  auto kern = verify_kernel<T>;
+  auto kern = verify_kernel<T, THREADS>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * parts));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -228,13 +316,22 @@ int sb_verify_drafts(const void* target, int64_t target_batch, int64_t target_ro
   a.d_s = draft_row;
   a.n_b = noise_batch;
   a.drafts = static_cast<int>(drafts);
-  // Eight CTAs (the portable cluster limit) while each keeps some rounds of loads.
+  // Eight CTAs (the portable cluster limit) while that is at most eight per SM (each
+  // starts with the dependent loads of the acceptance test: 256 sequences of 151936
+  // fp32 take 82 us with eight parts, 73.5 with four) and each keeps some rounds of loads.
   int parts = 8;
-  while (parts > 1 && v / parts < 2 * sb::verify::kThreads) parts /= 2;
+  while (parts > 1 && batch * parts > 8 * sb::device_sm_count()) parts /= 2;
+  while (parts > 1 && v / parts < 2048) parts /= 2;
   cudaStream_t st = sb::as_stream(stream);
-  if (dtype == SB_F32) return sb::verify::launch<float>(a, batch, parts, st);
-  if (dtype == SB_F16) return sb::verify::launch<__half>(a, batch, parts, st);
-  return sb::verify::launch<__nv_bfloat16>(a, batch, parts, st);
+  // Few sequences: a CTA has an SM to itself, and fewer rounds of loads end sooner.
+  const bool few = batch * parts <= sb::device_sm_count();
+  auto run = [&](auto type) {
+    using T = decltype(type);
+    return few ? sb::verify::launch<T, 1024>(a, batch, parts, st) : sb::verify::launch<T, 256>(a, batch, parts, st);
+  };
+  if (dtype == SB_F32) return run(float{});
+  if (dtype == SB_F16) return run(__half{});
+  return run(__nv_bfloat16{});
 }
 
 }  // extern "C"
