@@ -63,8 +63,7 @@ struct Params {
   int list;              // list length K
   const int* columns;    // [rows of the call, K] listed columns, rising
   const int* source;     // row of the call of each compact row
-  const uint16_t* starts;  // [2 n_tiles + 1, starts_ld] first list entry at or past column 128 j
-  int64_t starts_ld;
+  const uint16_t* starts;  // [rows of the call, 2 n_tiles + 1] first list entry at or past column 128 j
   float* listed;         // [compact rows, K] logits of the listed columns
   float2* stats;         // [2 n_tiles, rows_cap] exponent M and sum of 2^(y - M + 14)
   int store;             // write the exponentials too
@@ -150,6 +149,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two fp32 values in one 64-bit register pair: one instruction adds or scales both.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 values_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF16) {
@@ -170,13 +191,16 @@ constexpr float kLift = 14.0f;
 // in p.listed and count as absent; the others give the tile's exponent M (the maximum of
 // y = z log2(e) / tau rounded up) and sum of 2^(y - M + 14), which are also stored.
 template <bool BF16>
-__device__ __forceinline__ void logits_epilogue(const Params& p, float (&acc)[128], int row, int rows, int col0, int jt,
+__device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)[64], int row, int rows, int col0, int jt,
                                                 uint64_t lo, uint64_t hi, int entry, uint8_t* box,
                                                 const CUtensorMap* tm_out, int row_box, int lane) {
   const int ncol = p.cols - col0;
   if (ncol < 128) {
 #pragma unroll
-    for (int i = 0; i < 128; ++i) acc[i] = i < ncol ? acc[i] : -INFINITY;
+    for (int i = 0; i < 64; ++i) {
+      const float2 y = values_of(acc[i]);
+      acc[i] = pair_of(2 * i < ncol ? y.x : -INFINITY, 2 * i + 1 < ncol ? y.y : -INFINITY);
+    }
   }
   const bool valid = row < rows;
   float* listed = p.listed + (static_cast<int64_t>(p.row_base) + row) * p.list;
@@ -185,27 +209,44 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, float (&acc)[12
     const uint32_t word = static_cast<uint32_t>((c < 2 ? lo : hi) >> (32 * (c & 1)));
     if (word) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (word >> i & 1u) {
-          listed[entry++] = acc[32 * c + i];
-          acc[32 * c + i] = -INFINITY;
+      for (int i = 0; i < 16; ++i) {
+        if (word >> (2 * i) & 3u) {
+          float2 y = values_of(acc[16 * c + i]);
+          if (word >> (2 * i) & 1u) {
+            listed[entry++] = y.x;
+            y.x = -INFINITY;
+          }
+          if (word >> (2 * i) & 2u) {
+            listed[entry++] = y.y;
+            y.y = -INFINITY;
+          }
+          acc[16 * c + i] = pair_of(y.x, y.y);
         }
       }
     }
   }
-  float top[4] = {acc[0], acc[1], acc[2], acc[3]};
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], acc[i]);
+  for (int i = 0; i < 64; ++i) {
+    const float2 y = values_of(acc[i]);
+    top[i & 3] = fmaxf(fmaxf(top[i & 3], y.x), y.y);
+  }
   const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   const float m = t == -INFINITY ? 0.0f : ceilf(t * p.scale);
-  const float off = kLift - m;
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const uint64_t scale = pair_of(p.scale, p.scale), off = pair_of(kLift - m, kLift - m);
+  uint64_t s0 = 0, s1 = 0;
 #pragma unroll
-  for (int i = 0; i < 128; ++i) {
-    acc[i] = exp2_fast(fmaf(acc[i], p.scale, off));
-    s[i & 3] += acc[i];
+  for (int i = 0; i < 64; ++i) {
+    const float2 e = values_of(fma_pair(acc[i], scale, off));
+    acc[i] = pair_of(exp2_fast(e.x), exp2_fast(e.y));
+    if (i & 1) {
+      s1 = add_pair(s1, acc[i]);
+    } else {
+      s0 = add_pair(s0, acc[i]);
+    }
   }
-  if (valid) p.stats[static_cast<int64_t>(jt) * p.rows_cap + row] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+  const float2 s = values_of(add_pair(s0, s1));
+  if (valid) p.stats[static_cast<int64_t>(jt) * p.rows_cap + row] = make_float2(m, s.x + s.y);
   if (p.store) {
     const uint32_t swz = static_cast<uint32_t>(lane & 7);
 #pragma unroll
@@ -214,10 +255,14 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, float (&acc)[12
       __syncwarp();
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float* a = acc + panel * 64 + c * 8;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 e = values_of(acc[panel * 32 + c * 4 + j]);
+          w[j] = pack2<BF16>(e.x, e.y);
+        }
         *reinterpret_cast<uint4*>(box + lane * 128 + ((static_cast<uint32_t>(c) ^ swz) << 4)) =
-            make_uint4(pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3]), pack2<BF16>(a[4], a[5]),
-                       pack2<BF16>(a[6], a[7]));
+            make_uint4(w[0], w[1], w[2], w[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -230,7 +275,7 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, float (&acc)[12
 }
 
 // ---------------------------------------------------------------- product epilogue
-__device__ __forceinline__ void product_epilogue(const Params& p, float (&acc)[128], int col0, uint8_t* box,
+__device__ __forceinline__ void product_epilogue(const Params& p, uint64_t (&acc)[64], int col0, uint8_t* box,
                                                  const CUtensorMap* tm_out, int row_box, int lane) {
   const uint32_t swz = static_cast<uint32_t>(lane & 7);
 #pragma unroll
@@ -239,9 +284,9 @@ __device__ __forceinline__ void product_epilogue(const Params& p, float (&acc)[1
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float* a = acc + c * 32 + j * 4;
+      const float2 a = values_of(acc[c * 16 + j * 2]), b = values_of(acc[c * 16 + j * 2 + 1]);
       *reinterpret_cast<float4*>(box + lane * 128 + ((static_cast<uint32_t>(j) ^ swz) << 4)) =
-          make_float4(a[0], a[1], a[2], a[3]);
+          make_float4(a.x, a.y, b.x, b.y);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -415,10 +460,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int entry = 0;
       if constexpr (!PRODUCT) {
         if (row < rows) {
-          const int64_t at = static_cast<int64_t>(jt) * p.starts_ld + p.row_base + row;
-          entry = p.starts[at];
-          const int end = p.starts[at + p.starts_ld];
-          const int* columns = p.columns + static_cast<int64_t>(p.source[p.row_base + row]) * p.list;
+          const int64_t src = p.source[p.row_base + row];
+          const uint16_t* starts = p.starts + src * (2 * p.n_tiles + 1) + jt;
+          entry = starts[0];
+          const int end = starts[1];
+          const int* columns = p.columns + src * p.list;
           for (int e = entry; e < end; ++e) {
             const int c = columns[e] - col0;
             if (c < 64) {
@@ -429,9 +475,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      float acc[128];
+      uint64_t acc[64];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < 64; ++i) acc[i] = 0;
 #pragma unroll 1
       for (int kb = u.k0; kb < u.k1; kb += p.seg, ++accs) {
         const uint32_t buf = accs & 1;
@@ -442,13 +488,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t tacc = tlane + buf * kTile;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld32(tacc + c * 32, v);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32], w[32];
+          tmem_ld32(tacc + c * 64, v);
+          tmem_ld32(tacc + c * 64 + 32, w);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            acc[32 * c + i] += __uint_as_float(v[i]);
+          for (int i = 0; i < 16; ++i) {
+            acc[32 * c + i] = add_pair(acc[32 * c + i], pair_of(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
+            acc[32 * c + 16 + i] =
+                add_pair(acc[32 * c + 16 + i], pair_of(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])));
           }
         }
         tc_fence_before();

@@ -77,15 +77,16 @@ __global__ void check_kernel(const int64_t* __restrict__ indices, int64_t rows, 
   if (repeats) atomicAdd(&faults[1], repeats);
 }
 
-// One warp per row: the used entries sorted by column, log p of each, p_rest, and how
-// many are used (0 leaves the row out).  K <= 256: an entry's place is the number of
-// entries before it.
+// One warp per row: the used entries sorted by column, log p of each, p_rest, how many
+// are used (0 leaves the row out), and each tile's first entry.  K <= 256: an entry's
+// place is the number of entries before it.
 template <typename T>
 __global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict__ indices, const void* __restrict__ logits,
                                                       const float* __restrict__ lse, int64_t rows, int k, int64_t v,
-                                                      float inv_tau, int* __restrict__ columns, float* __restrict__ logp,
-                                                      float* __restrict__ rest, int* __restrict__ used) {
-  __shared__ int s_col[4][kMaxList];
+                                                      float inv_tau, int tiles, int* __restrict__ columns,
+                                                      float* __restrict__ logp, float* __restrict__ rest,
+                                                      int* __restrict__ used, uint16_t* __restrict__ starts) {
+  __shared__ int s_col[4][kMaxList], s_sorted[4][kMaxList];
   __shared__ float s_t[4][kMaxList];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict_
     for (int i = 0; i < k; ++i) place += (col[i] < c || (col[i] == c && i < j)) ? 1 : 0;
     const float lp = c == kNone ? -INFINITY : tv[j] - norm;
     columns[row * k + place] = c;
+    s_sorted[warp][place] = c;
     logp[row * k + place] = lp;
     if (c != kNone) sum += expf(lp);
   }
@@ -133,78 +135,61 @@ __global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict_
     rest[row] = !lse || n == v ? 0.0f : (left < 0.0f ? 0.0f : left);
     used[row] = n;
   }
+  if (n == 0) return;
+  __syncwarp();
+  // For each 128-column tile the first entry at or past it (unused ones lie past all).
+  const int* sorted = s_sorted[warp];
+  const int first_o = 1 << (31 - __clz(k));
+  for (int j = lane; j <= tiles; j += 32) {
+    const int64_t from = static_cast<int64_t>(j) * 128;
+    int below = 0;
+    for (int o = first_o; o; o >>= 1) below += below + o <= k && sorted[below + o - 1] < from ? o : 0;
+    starts[row * (tiles + 1) + j] = static_cast<uint16_t>(below);
+  }
 }
 
-// Compact order of the rows that have a list (one block; the order is the rows').
-__global__ void __launch_bounds__(1024) compact_kernel(const int* __restrict__ used, int64_t rows, int* __restrict__ source,
-                                                       int* __restrict__ place, int* __restrict__ count) {
-  __shared__ int s_warp[32];
+// 32 rows per CTA: the compact order of the rows that have a list (the rows' own order:
+// each CTA counts those before it), their hidden states gathered, zero loss and mass for
+// the others.
+__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ hidden, int64_t h,
+                                                     const int* __restrict__ used, int64_t rows, int* __restrict__ source,
+                                                     int* __restrict__ place, int* __restrict__ count,
+                                                     uint16_t* __restrict__ out, float* __restrict__ loss,
+                                                     float* __restrict__ mass) {
+  __shared__ int s_warp[8], s_place[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int base = 0;
-  for (int64_t start = 0; start < rows; start += 1024) {
-    const int64_t i = start + threadIdx.x;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 32;
+  int before = 0;
+  for (int64_t i = threadIdx.x; i < r0; i += 256) before += used[i] > 0 ? 1 : 0;
+  for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) s_warp[warp] = before;
+  __syncthreads();
+  if (warp == 0) {
+    int base = lane < 8 ? s_warp[lane] : 0;
+    for (int o = 16; o; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+    const int64_t i = r0 + lane;
     const bool in = i < rows && used[i] > 0;
     const unsigned votes = __ballot_sync(0xffffffffu, in);
-    if (lane == 0) s_warp[warp] = __popc(votes);
-    __syncthreads();
-    int mine = s_warp[lane];
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, mine, o);
-      if (lane >= o) mine += up;
-    }
-    const int before = __shfl_sync(0xffffffffu, mine, (warp + 31) & 31);
-    const int total = __shfl_sync(0xffffffffu, mine, 31);
-    const int at = base + (warp ? before : 0) + __popc(votes & ((1u << lane) - 1u));
+    const int at = base + __popc(votes & ((1u << lane) - 1u));
+    s_place[lane] = in ? at : -1;
     if (i < rows) {
       place[i] = in ? at : -1;
-      if (in) source[at] = static_cast<int>(i);
+      if (in) {
+        source[at] = static_cast<int>(i);
+      } else {
+        loss[i] = 0.0f;
+        mass[i] = 0.0f;
+      }
     }
-    base += total;
-    __syncthreads();
+    if (lane == 0 && r0 + 32 >= rows) *count = base + __popc(votes);
   }
-  if (threadIdx.x == 0) *count = base;
-}
-
-// 32 compact rows per CTA: their hidden states gathered, and for each row and 128-column
-// tile the first list entry at or past it.
-__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ hidden, int64_t h,
-                                                     const int* __restrict__ source, const int* __restrict__ count,
-                                                     const int* __restrict__ columns, int k, int tiles, int64_t ld,
-                                                     uint16_t* __restrict__ out, uint16_t* __restrict__ starts,
-                                                     float* __restrict__ loss, float* __restrict__ mass,
-                                                     const int* __restrict__ used, int64_t rows) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c0 = static_cast<int64_t>(blockIdx.x) * 32;
-  if (warp == 0) {  // rows left out: zero loss and mass
-    const int64_t i = c0 + lane;
-    if (i < rows && used[i] == 0) {
-      loss[i] = 0.0f;
-      mass[i] = 0.0f;
-    }
-  }
-  const int n = *count;
-  if (c0 >= n) return;
-  for (int r = warp; r < 32 && c0 + r < n; r += 8) {
-    const uint4* from = reinterpret_cast<const uint4*>(hidden + static_cast<int64_t>(source[c0 + r]) * h);
-    uint4* to = reinterpret_cast<uint4*>(out + (c0 + r) * h);
+  __syncthreads();
+  for (int r = warp; r < 32; r += 8) {
+    const int at = s_place[r];
+    if (at < 0) continue;
+    const uint4* from = reinterpret_cast<const uint4*>(hidden + (r0 + r) * h);
+    uint4* to = reinterpret_cast<uint4*>(out + at * h);
     for (int64_t i = lane; i < h / 8; i += 32) to[i] = from[i];
-  }
-  const int64_t c = c0 + lane;
-  if (c >= n) return;
-  const int* list = columns + static_cast<int64_t>(source[c]) * k;
-  const int per = (tiles + 1 + 7) / 8;
-  const int j0 = warp * per, j1 = j0 + per < tiles + 1 ? j0 + per : tiles + 1;
-  if (j0 >= j1) return;
-  int lo = 0, hi = k;  // first entry with column >= 128 j0
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (list[mid] < static_cast<int64_t>(j0) * 128) lo = mid + 1; else hi = mid;
-  }
-  int next = lo < k ? list[lo] : kNone;
-  for (int j = j0; j < j1; ++j) {
-    while (next < static_cast<int64_t>(j) * 128) next = ++lo < k ? list[lo] : kNone;
-    // Unused entries (kNone) lie past every tile: the last start counts used ones only.
-    starts[static_cast<int64_t>(j) * ld + c] = static_cast<uint16_t>(lo);
   }
 }
 
@@ -231,6 +216,13 @@ __device__ __forceinline__ float gap(float p, float logp, float q, float logq) {
 // so only the listed columns' values are rounded anew, and is such that neither passes
 // 2^15 in fp16.
 constexpr int kMergeThreads = 1024;
+constexpr float kLow = -1e9f;  // below every exponent
+
+// 2^x for a whole x <= 0 (zero below -126; NaN stays).
+__device__ __forceinline__ float power(float x) {
+  return x > -127.0f ? __int_as_float((static_cast<int>(x) + 127) << 23) : (x == x ? 0.0f : x);
+}
+
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
     const float2* __restrict__ stats, int64_t ld, int tiles, const int* __restrict__ count, int row_base,
     const int* __restrict__ source, const int* __restrict__ used, const float* __restrict__ logp,
@@ -241,16 +233,25 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
   const int r = threadIdx.x & 7, g = threadIdx.x >> 3;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + r;
   if (static_cast<int64_t>(blockIdx.x) * 8 >= n) return;
-  float R = -1e30f, S = 0.0f;
+  float R = kLow, S = 0.0f;
   if (row < n) {
-    for (int j = g; j < tiles; j += kMergeThreads / 8) {
-      const float2 t = stats[j * ld + row];
-      if (t.y == 0.0f) continue;
-      if (t.x > R) {
-        S *= exp2f(R - t.x);
-        R = t.x;
+    // Loads first, several at a time; every factor is a power of two (exact).
+    constexpr int kAtOnce = 10;
+    for (int j0 = g; j0 < tiles; j0 += kAtOnce * (kMergeThreads / 8)) {
+      float2 t[kAtOnce];
+      float top = R;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int64_t j = j0 + i * (kMergeThreads / 8);
+        t[i] = j < tiles ? stats[j * ld + row] : make_float2(kLow, 0.0f);
+        if (t[i].y != 0.0f) top = fmaxf(top, t[i].x);
       }
-      S += t.y * exp2f(t.x - R);  // a power of two: exact
+      S *= power(R - top);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (t[i].y != 0.0f) S += t[i].y * power(t[i].x - top);
+      }
+      R = top;
     }
   }
   s_r[threadIdx.x] = R;
@@ -260,13 +261,13 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
   if (warp >= 8) return;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + warp;
   if (at >= n) return;
-  R = -1e30f;
+  R = kLow;
   S = 0.0f;
   for (int i = lane; i < kMergeThreads / 8; i += 32) R = fmaxf(R, s_r[i * 8 + warp]);
   R = warp_max(R);
   for (int i = lane; i < kMergeThreads / 8; i += 32) {
     const float s = s_s[i * 8 + warp];
-    if (s != 0.0f) S += s * exp2f(s_r[i * 8 + warp] - R);
+    if (s != 0.0f) S += s * power(s_r[i * 8 + warp] - R);
   }
   S = warp_sum(S) * exp2f(-dense::kLift);
   const int64_t src = source[row_base + at];
@@ -491,13 +492,9 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
   const float scale = kLog2e / temperature;
   const int pairs = device_sm_count() / 2;
 
-  compact_kernel<<<1, 1024, 0, st>>>(used, t, source, place, count);
+  gather_kernel<<<static_cast<unsigned>((t + 31) / 32), 256, 0, st>>>(hidden, h, used, t, source, place, count, hc, loss, mass);
   count_launch();
-  gather_kernel<<<static_cast<unsigned>((t + 31) / 32), 256, 0, st>>>(hidden, h, source, count, columns, k,
-                                                                       static_cast<int>(L.tiles), t, hc, starts, loss, mass,
-                                                                       used, t);
-  count_launch();
-  if (int rc = check_launch("distill compact")) return rc;
+  if (int rc = check_launch("distill gather")) return rc;
   CUtensorMap m_w;
   int rc = make_map(&m_w, dt, weight, h, v, h * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
@@ -514,13 +511,14 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
     p.cols = static_cast<int>(v);
     p.n_tiles = L.n_tiles;
     p.k_blocks = static_cast<int>((h + 63) / 64);
-    p.seg = 4;
+    // At most six k-blocks (384 products) per accumulation, in runs of even length.
+    const int runs = (p.k_blocks + 5) / 6;
+    p.seg = (p.k_blocks + runs - 1) / runs;
     p.scale = scale;
     p.list = k;
     p.columns = columns;
     p.source = source;
     p.starts = starts;
-    p.starts_ld = t;
     p.listed = listed;
     p.stats = stats;
     p.store = train ? 1 : 0;
@@ -613,8 +611,9 @@ int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint1
                  : logits_dtype == SB_F16 ? prepare_kernel<__half>
                                           : prepare_kernel<__nv_bfloat16>;
   prepare<<<static_cast<unsigned>((t + 3) / 4), 128, 0, st>>>(
-      indices, logits, teacher_lse, t, k, v, 1.0f / temperature, reinterpret_cast<int*>(ws + L.columns),
-      reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest), reinterpret_cast<int*>(ws + L.used));
+      indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), reinterpret_cast<int*>(ws + L.columns),
+      reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest), reinterpret_cast<int*>(ws + L.used),
+      reinterpret_cast<uint16_t*>(ws + L.starts));
   sb::count_launch();
   if (int rc = sb::check_launch("distill prepare")) return rc;
   return dtype == SB_BF16
