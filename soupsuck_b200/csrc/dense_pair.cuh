@@ -62,8 +62,7 @@ struct Params {
   float scale;           // log2(e) / temperature
   int list;              // list length K
   const int* columns;    // [rows of the call, K] listed columns, rising
-  const int* source;     // row of the call of each compact row
-  const uint16_t* starts;  // [rows of the call, 2 n_tiles + 1] first list entry at or past column 128 j
+  const uint32_t* lookup;  // [compact rows, 2 n_tiles] which columns of each 128 are listed (listed_word)
   float* listed;         // [compact rows, K] logits of the listed columns
   float2* stats;         // [2 n_tiles, rows_cap] exponent M and sum of 2^(y - M + 14)
   int store;             // write the exponentials too
@@ -186,14 +185,26 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // to a power of two), so fp16 keeps its 11 bits down to 2^-28 of it.
 constexpr float kLift = 14.0f;
 
+// The list entries of one row in one tile of 128 columns: columns of the first three (7
+// bits each), the first one's number in the list (8), how many (2, at most 3), whether
+// there are more (1).  One load per row and tile; finding them from the list itself was
+// three dependent ones, a tenth of the kernel.
+__device__ __forceinline__ uint32_t listed_word(int first, int n, int c0, int c1, int c2) {
+  uint32_t w = static_cast<uint32_t>(first & 255) << 21 | static_cast<uint32_t>(n < 3 ? n : 3) << 29 | (n > 3 ? 1u << 31 : 0u);
+  if (n > 0) w |= static_cast<uint32_t>(c0 & 127);
+  if (n > 1) w |= static_cast<uint32_t>(c1 & 127) << 7;
+  if (n > 2) w |= static_cast<uint32_t>(c2 & 127) << 14;
+  return w;
+}
+
 // ---------------------------------------------------------------- logits epilogue
 // acc: this thread's row, columns col0 .. col0 + 127.  Listed columns leave their logit
 // in p.listed and count as absent; the others give the tile's exponent M (the maximum of
 // y = z log2(e) / tau rounded up) and sum of 2^(y - M + 14), which are also stored.
 template <bool BF16>
 __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)[64], int row, int rows, int col0, int jt,
-                                                uint64_t lo, uint64_t hi, int entry, uint8_t* box,
-                                                const CUtensorMap* tm_out, int row_box, int lane) {
+                                                uint32_t listed_here, uint8_t* box, const CUtensorMap* tm_out, int row_box,
+                                                int lane) {
   const int ncol = p.cols - col0;
   if (ncol < 128) {
 #pragma unroll
@@ -203,7 +214,25 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)
     }
   }
   const bool valid = row < rows;
-  float* listed = p.listed + (static_cast<int64_t>(p.row_base) + row) * p.list;
+  const int64_t list_at = (static_cast<int64_t>(p.row_base) + row) * p.list;
+  float* listed = p.listed + list_at;
+  int entry = (listed_here >> 21) & 255;
+  uint64_t lo = 0, hi = 0;
+  {
+    const int n = (listed_here >> 29) & 3;
+    auto mark = [&](int c) {
+      const uint64_t bit = 1ull << (c & 63);
+      lo |= c < 64 ? bit : 0;
+      hi |= c < 64 ? 0 : bit;
+    };
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      if (e < n) mark((listed_here >> (7 * e)) & 127);
+    }
+    if (listed_here >> 31) {
+      for (int e = entry + 3; e < p.list && p.columns[list_at + e] < col0 + 128; ++e) mark(p.columns[list_at + e] & 127);
+    }
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const uint32_t word = static_cast<uint32_t>((c < 2 ? lo : hi) >> (32 * (c & 1)));
@@ -455,25 +484,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row = row_box + lane;
       const int col0 = u.nt * kTile + half * kHalf;
       const int jt = u.nt * 2 + half;
-      // Which of this thread's 128 columns are listed (read while the tile accumulates).
-      uint64_t lo = 0, hi = 0;
-      int entry = 0;
+      uint32_t listed_here = 0;
       if constexpr (!PRODUCT) {
-        if (row < rows) {
-          const int64_t src = p.source[p.row_base + row];
-          const uint16_t* starts = p.starts + src * (2 * p.n_tiles + 1) + jt;
-          entry = starts[0];
-          const int end = starts[1];
-          const int* columns = p.columns + src * p.list;
-          for (int e = entry; e < end; ++e) {
-            const int c = columns[e] - col0;
-            if (c < 64) {
-              lo |= 1ull << c;
-            } else {
-              hi |= 1ull << (c - 64);
-            }
-          }
-        }
+        if (row < rows) listed_here = p.lookup[(static_cast<int64_t>(p.row_base) + row) * (2 * p.n_tiles) + jt];
       }
       uint64_t acc[64];
 #pragma unroll
@@ -508,7 +521,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if constexpr (PRODUCT) {
         product_epilogue(p, acc, col0, box, &tm_out, u.split * units.m_tiles * kTile + row_box, lane);
       } else {
-        logits_epilogue<BF16>(p, acc, row, rows, col0, jt, lo, hi, entry, box, &tm_out, row_box, lane);
+        logits_epilogue<BF16>(p, acc, row, rows, col0, jt, listed_here, box, &tm_out, row_box, lane);
       }
     }
     if (lane == 0) bulk_wait_all();

@@ -11,8 +11,8 @@
 // The -p + q terms sum to zero over both distributions; with them every term is at
 // least zero and nothing cancels where student and teacher are close.
 //
-// Forward.  prepare sorts each row's list and computes log p; rows without a listed
-// column are left out of everything else (compact).  One tensor-core launch forms the
+// Forward.  prepare gathers the answered rows (the others are left out of everything
+// else), sorts each one's list and computes log p.  One tensor-core launch forms the
 // logits tile by tile (dense_pair.cuh): listed ones are written out, the others leave a
 // power-of-two exponent and a sum of exponentials per row and 128 columns, and, where a
 // gradient is wanted, the exponentials themselves in 16 bits [rows, V].  merge joins them
@@ -77,32 +77,89 @@ __global__ void check_kernel(const int64_t* __restrict__ indices, int64_t rows, 
   if (repeats) atomicAdd(&faults[1], repeats);
 }
 
-// One warp per row: the used entries sorted by column, log p of each, p_rest, how many
-// are used (0 leaves the row out), and each tile's first entry.  K <= 256: an entry's
-// place is the number of entries before it.
+// Which rows are answered: a listed column, and on the list some teacher probability.
+// One warp per row; `blocks` counts the answered rows of each CTA's eight.
+constexpr int kRowsPerBlock = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict__ indices, const void* __restrict__ logits,
-                                                      const float* __restrict__ lse, int64_t rows, int k, int64_t v,
-                                                      float inv_tau, int tiles, int* __restrict__ columns,
-                                                      float* __restrict__ logp, float* __restrict__ rest,
-                                                      int* __restrict__ used, uint16_t* __restrict__ starts) {
-  __shared__ int s_col[4][kMaxList], s_sorted[4][kMaxList];
-  __shared__ float s_t[4][kMaxList];
+__global__ void __launch_bounds__(256) answered_kernel(const int64_t* __restrict__ indices, const void* __restrict__ logits,
+                                                       const float* __restrict__ lse, int64_t rows, int k, int64_t v,
+                                                       int* __restrict__ place, int* __restrict__ blocks) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
+  bool some = false;
+  if (row < rows) {
+    for (int j = lane; j < k; j += 32) {
+      const int64_t c = indices[row * k + j];
+      some |= c >= 0 && c < v && (lse || !(logit_at<T>(logits, row * k + j) == -INFINITY));
+    }
+    some = __any_sync(0xffffffffu, some) && !(lse && lse[row] == -INFINITY);
+    if (lane == 0) place[row] = some ? 1 : -1;
+  }
+  const int n = __syncthreads_count(some && lane == 0);
+  if (threadIdx.x == 0) blocks[blockIdx.x] = n;
+}
+
+// What the other kernels need of each answered row, in the rows' order without gaps: its
+// hidden state, its list sorted by column, log p of each entry, p_rest, how many entries
+// are used, and which entries each 128-column tile has.  Rows that are not answered get zero
+// loss and mass here.  One warp per row; an entry's place is the number of entries
+// before it (K <= 256).
+template <typename T>
+__global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict__ hidden, int64_t h,
+                                                      const int64_t* __restrict__ indices, const void* __restrict__ logits,
+                                                      const float* __restrict__ lse, int64_t rows, int k, int64_t v,
+                                                      float inv_tau, int tiles, const int* __restrict__ blocks,
+                                                      int* __restrict__ place, int* __restrict__ source,
+                                                      int* __restrict__ count, uint16_t* __restrict__ gathered,
+                                                      int* __restrict__ columns, float* __restrict__ logp,
+                                                      float* __restrict__ rest, int* __restrict__ used,
+                                                      uint32_t* __restrict__ lookup, float* __restrict__ loss,
+                                                      float* __restrict__ mass) {
+  __shared__ int s_col[kRowsPerBlock][kMaxList];
+  __shared__ float s_t[kRowsPerBlock][kMaxList];
+  __shared__ int s_before[kRowsPerBlock], s_in[kRowsPerBlock];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
+  int before = 0;
+  for (int i = threadIdx.x; i < static_cast<int>(blockIdx.x); i += 256) before += blocks[i];
+  for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  const bool in = row < rows && place[row] > 0;
+  if (lane == 0) {
+    s_before[warp] = before;
+    s_in[warp] = in ? 1 : 0;
+  }
+  __syncthreads();
+  int at = 0;
+  for (int i = 0; i < kRowsPerBlock; ++i) at += s_before[i] + (i < warp ? s_in[i] : 0);
+  if (lane == 0 && warp == kRowsPerBlock - 1 && blockIdx.x == gridDim.x - 1) *count = at + s_in[warp];
   if (row >= rows) return;
+  if (lane == 0) {
+    place[row] = in ? at : -1;
+    if (in) {
+      source[at] = static_cast<int>(row);
+    } else {
+      loss[row] = 0.0f;
+      mass[row] = 0.0f;
+    }
+  }
+  if (!in) return;
+  {
+    const uint4* from = reinterpret_cast<const uint4*>(hidden + row * h);
+    uint4* to = reinterpret_cast<uint4*>(gathered + at * h);
+    for (int64_t i = lane; i < h / 8; i += 32) to[i] = from[i];
+  }
   int* col = s_col[warp];
   float* tv = s_t[warp];
   int n = 0;
   float top = -INFINITY;
   for (int j = lane; j < k; j += 32) {
     const int64_t c = indices[row * k + j];
-    const bool in = c >= 0 && c < v;
-    const float t = in ? logit_at<T>(logits, row * k + j) * inv_tau : -INFINITY;
-    col[j] = in ? static_cast<int>(c) : kNone;
+    const bool used_here = c >= 0 && c < v;
+    const float t = used_here ? logit_at<T>(logits, row * k + j) * inv_tau : -INFINITY;
+    col[j] = used_here ? static_cast<int>(c) : kNone;
     tv[j] = t;
-    n += in ? 1 : 0;
-    top = t == t ? fmaxf(top, t) : INFINITY;  // a NaN keeps the row, and makes it NaN
+    n += used_here ? 1 : 0;
+    top = t == t ? fmaxf(top, t) : INFINITY;  // a NaN makes the row NaN
   }
   for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   top = warp_max(top);
@@ -111,85 +168,43 @@ __global__ void __launch_bounds__(128) prepare_kernel(const int64_t* __restrict_
   float norm;
   if (lse) {
     norm = lse[row];
-    if (norm == -INFINITY) n = 0;
   } else {
     float s = 0.0f;
     for (int j = lane; j < k; j += 32) s += expf(tv[j] - top);
     norm = top + logf(warp_sum(s));
   }
-  if (top == -INFINITY && !lse) n = 0;  // no teacher mass on the list
+  int* row_columns = columns + static_cast<int64_t>(at) * k;
+  float* row_logp = logp + static_cast<int64_t>(at) * k;
   float sum = 0.0f;
   for (int j = lane; j < k; j += 32) {
     const int c = col[j];
-    int place = 0;
-    for (int i = 0; i < k; ++i) place += (col[i] < c || (col[i] == c && i < j)) ? 1 : 0;
+    int where = 0;
+    for (int i = 0; i < k; ++i) where += (col[i] < c || (col[i] == c && i < j)) ? 1 : 0;
     const float lp = c == kNone ? -INFINITY : tv[j] - norm;
-    columns[row * k + place] = c;
-    s_sorted[warp][place] = c;
-    logp[row * k + place] = lp;
+    row_columns[where] = c;
+    row_logp[where] = lp;
     if (c != kNone) sum += expf(lp);
   }
   sum = warp_sum(sum);
   if (lane == 0) {
     const float left = 1.0f - sum;
-    rest[row] = !lse || n == v ? 0.0f : (left < 0.0f ? 0.0f : left);
-    used[row] = n;
+    rest[at] = !lse || n == v ? 0.0f : (left < 0.0f ? 0.0f : left);
+    used[at] = n;
   }
-  if (n == 0) return;
+  // The tiles' lookups: zeros, then each tile's from its first entry.
+  uint32_t* row_lookup = lookup + static_cast<int64_t>(at) * tiles;
+  for (int j = lane; j < tiles / 2; j += 32) reinterpret_cast<uint2*>(row_lookup)[j] = make_uint2(0u, 0u);
   __syncwarp();
-  // For each 128-column tile the first entry at or past it (unused ones lie past all).
-  const int* sorted = s_sorted[warp];
-  const int first_o = 1 << (31 - __clz(k));
-  for (int j = lane; j <= tiles; j += 32) {
-    const int64_t from = static_cast<int64_t>(j) * 128;
-    int below = 0;
-    for (int o = first_o; o; o >>= 1) below += below + o <= k && sorted[below + o - 1] < from ? o : 0;
-    starts[row * (tiles + 1) + j] = static_cast<uint16_t>(below);
-  }
-}
-
-// 32 rows per CTA: the compact order of the rows that have a list (the rows' own order:
-// each CTA counts those before it), their hidden states gathered, zero loss and mass for
-// the others.
-__global__ void __launch_bounds__(256) gather_kernel(const uint16_t* __restrict__ hidden, int64_t h,
-                                                     const int* __restrict__ used, int64_t rows, int* __restrict__ source,
-                                                     int* __restrict__ place, int* __restrict__ count,
-                                                     uint16_t* __restrict__ out, float* __restrict__ loss,
-                                                     float* __restrict__ mass) {
-  __shared__ int s_warp[8], s_place[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 32;
-  int before = 0;
-  for (int64_t i = threadIdx.x; i < r0; i += 256) before += used[i] > 0 ? 1 : 0;
-  for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (lane == 0) s_warp[warp] = before;
-  __syncthreads();
-  if (warp == 0) {
-    int base = lane < 8 ? s_warp[lane] : 0;
-    for (int o = 16; o; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
-    const int64_t i = r0 + lane;
-    const bool in = i < rows && used[i] > 0;
-    const unsigned votes = __ballot_sync(0xffffffffu, in);
-    const int at = base + __popc(votes & ((1u << lane) - 1u));
-    s_place[lane] = in ? at : -1;
-    if (i < rows) {
-      place[i] = in ? at : -1;
-      if (in) {
-        source[at] = static_cast<int>(i);
-      } else {
-        loss[i] = 0.0f;
-        mass[i] = 0.0f;
-      }
+  for (int j = lane; j < n; j += 32) {
+    const int c = row_columns[j], tile = c >> 7;
+    if (j > 0 && row_columns[j - 1] >> 7 == tile) continue;
+    int next[3], here = 1;
+#pragma unroll
+    for (int e = 0; e < 3; ++e) {
+      next[e] = j + 1 + e < n ? row_columns[j + 1 + e] : kNone;
+      here += next[e] >> 7 == tile ? 1 : 0;
     }
-    if (lane == 0 && r0 + 32 >= rows) *count = base + __popc(votes);
-  }
-  __syncthreads();
-  for (int r = warp; r < 32; r += 8) {
-    const int at = s_place[r];
-    if (at < 0) continue;
-    const uint4* from = reinterpret_cast<const uint4*>(hidden + (r0 + r) * h);
-    uint4* to = reinterpret_cast<uint4*>(out + at * h);
-    for (int64_t i = lane; i < h / 8; i += 32) to[i] = from[i];
+    row_lookup[tile] = dense::listed_word(j, here, c, next[0], next[1]);
   }
 }
 
@@ -208,14 +223,14 @@ __device__ __forceinline__ float gap(float p, float logp, float q, float logq) {
   return q * (r * expf(r) - expm1f(r));
 }
 
-// Eight rows per CTA.  Joins a row's tile statistics and listed logits into its loss and
+// Four rows per CTA.  Joins a row's tile statistics and listed logits into its loss and
 // mass, and for the gradient: `shift` so that a tile's exponentials times 2^(M + shift)
 // are dz in the row's unit, `unit` (dz's factor), and the listed columns' dz / unit (over
 // their logits).  The unit is a power of two times the factor all unlisted columns share,
 //   b = 2^(R - lse2) - p_rest / S     (R the largest M, S the sum of 2^(y - R)),
 // so only the listed columns' values are rounded anew, and is such that neither passes
 // 2^15 in fp16.
-constexpr int kMergeThreads = 1024;
+constexpr int kMergeThreads = 512, kMergeRows = 4;
 constexpr float kLow = -1e9f;  // below every exponent
 
 // 2^x for a whole x <= 0 (zero below -126; NaN stays).
@@ -230,19 +245,20 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
     float* __restrict__ mass, float* __restrict__ unit, int* __restrict__ shift) {
   __shared__ float s_r[kMergeThreads], s_s[kMergeThreads];
   const int n = *count - row_base;
-  const int r = threadIdx.x & 7, g = threadIdx.x >> 3;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + r;
-  if (static_cast<int64_t>(blockIdx.x) * 8 >= n) return;
+  const int r = threadIdx.x % kMergeRows, g = threadIdx.x / kMergeRows;
+  constexpr int kGroups = kMergeThreads / kMergeRows;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeRows + r;
+  if (static_cast<int64_t>(blockIdx.x) * kMergeRows >= n) return;
   float R = kLow, S = 0.0f;
   if (row < n) {
     // Loads first, several at a time; every factor is a power of two (exact).
     constexpr int kAtOnce = 10;
-    for (int j0 = g; j0 < tiles; j0 += kAtOnce * (kMergeThreads / 8)) {
+    for (int j0 = g; j0 < tiles; j0 += kAtOnce * kGroups) {
       float2 t[kAtOnce];
       float top = R;
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
-        const int64_t j = j0 + i * (kMergeThreads / 8);
+        const int64_t j = j0 + i * kGroups;
         t[i] = j < tiles ? stats[j * ld + row] : make_float2(kLow, 0.0f);
         if (t[i].y != 0.0f) top = fmaxf(top, t[i].x);
       }
@@ -258,22 +274,22 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
   s_s[threadIdx.x] = S;
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp >= 8) return;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  if (warp >= kMergeRows) return;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kMergeRows + warp;
   if (at >= n) return;
   R = kLow;
   S = 0.0f;
-  for (int i = lane; i < kMergeThreads / 8; i += 32) R = fmaxf(R, s_r[i * 8 + warp]);
+  for (int i = lane; i < kGroups; i += 32) R = fmaxf(R, s_r[i * kMergeRows + warp]);
   R = warp_max(R);
-  for (int i = lane; i < kMergeThreads / 8; i += 32) {
-    const float s = s_s[i * 8 + warp];
-    if (s != 0.0f) S += s * power(s_r[i * 8 + warp] - R);
+  for (int i = lane; i < kGroups; i += 32) {
+    const float s = s_s[i * kMergeRows + warp];
+    if (s != 0.0f) S += s * power(s_r[i * kMergeRows + warp] - R);
   }
   S = warp_sum(S) * exp2f(-dense::kLift);
   const int64_t src = source[row_base + at];
-  const int m = used[src];
+  const int m = used[row_base + at];
   float* z = listed + (row_base + at) * k;
-  const float* lp = logp + src * k;
+  const float* lp = logp + (row_base + at) * k;
   float top = S > 0.0f ? R : -INFINITY;
   for (int j = lane; j < m; j += 32) top = fmaxf(top, z[j] * scale);
   top = warp_max(top);
@@ -295,7 +311,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
   gaps = warp_sum(gaps);
   covered = warp_sum(covered);
   largest = warp_max(largest);
-  const float p_rest = rest[src];
+  const float p_rest = rest[row_base + at];
   const float head = exp2f(R - lse2);
   if (lane == 0) {
     if (S > 0.0f || !(S == S)) gaps += gap(p_rest, logf(p_rest), S * head, (R - lse2 + log2f(S)) * kLn2);
@@ -329,8 +345,7 @@ constexpr int kScaleThreads = 256, kScaleVecs = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(kScaleThreads) scale_kernel(
     uint16_t* __restrict__ dz, int64_t pitch, const float2* __restrict__ stats, int64_t ld, const int* __restrict__ count,
-    int row_base, const int* __restrict__ source, const int* __restrict__ used, const int* __restrict__ columns,
-    const float* __restrict__ listed, int k, const int* __restrict__ shift) {
+    int row_base, const int* __restrict__ used, const int* __restrict__ columns, const float* __restrict__ listed, int k, const int* __restrict__ shift) {
   const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 32768;
   if (row >= *count - row_base || row >= ld) return;
   const int e = shift[row_base + row];
@@ -360,10 +375,9 @@ __global__ void __launch_bounds__(kScaleThreads) scale_kernel(
   }
   __syncthreads();
   const int64_t c0 = v0 * 8, c1 = c0 + kScaleThreads * kScaleVecs * 8;
-  const int64_t src = source[row_base + row];
-  const int n = used[src];
+  const int n = used[row_base + row];
   for (int j = threadIdx.x; j < n; j += kScaleThreads) {
-    const int c = columns[src * k + j];
+    const int c = columns[(row_base + row) * k + j];
     if (c >= c0 && c < c1) {
       line[c] = static_cast<uint16_t>(dense::pack2<BF16>(listed[(row_base + row) * k + j], 0.0f) & 0xffffu);
     }
@@ -418,7 +432,7 @@ __global__ void __launch_bounds__(256) backward_kernel(const float* __restrict__
 struct Layout {
   int64_t tiles, pitch, cap, room;
   int n_tiles, out_tiles, k_blocks;
-  size_t columns, logp, listed, rest, used, source, count, unit, shift, hidden, starts, stats, dz, parts, total;
+  size_t columns, logp, listed, rest, used, source, blocks, count, unit, shift, hidden, lookup, stats, dz, parts, total;
 };
 
 inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
@@ -446,11 +460,12 @@ inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
   L.rest = take(t * 4);
   L.used = take(t * 4);
   L.source = take(t * 4);
+  L.blocks = take((t + kRowsPerBlock - 1) / kRowsPerBlock * 4);
   L.count = take(16);
   L.unit = take(t * 4);
   L.shift = take(t * 4);
   L.hidden = take(t * h * 2);
-  L.starts = take((L.tiles + 1) * t * 2);
+  L.lookup = take(L.tiles * t * 4);
   L.stats = take(L.tiles * L.cap * 8);
   if (train) {
     L.dz = take(L.cap * L.pitch * 2);
@@ -469,8 +484,8 @@ inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
 }
 
 template <bool BF16>
-int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, float temperature,
-            const Layout& L, uint8_t* ws, float* loss, float* mass, float* du, int* place, cudaStream_t st) {
+int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, float temperature, const Layout& L, uint8_t* ws,
+            float* loss, float* mass, float* du, cudaStream_t st) {
   using namespace gemm;
   auto ptr = [&](size_t at) { return ws + at; };
   int* columns = reinterpret_cast<int*>(ptr(L.columns));
@@ -483,7 +498,7 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
   float* unit = reinterpret_cast<float*>(ptr(L.unit));
   int* shift = reinterpret_cast<int*>(ptr(L.shift));
   uint16_t* hc = reinterpret_cast<uint16_t*>(ptr(L.hidden));
-  uint16_t* starts = reinterpret_cast<uint16_t*>(ptr(L.starts));
+  uint32_t* lookup = reinterpret_cast<uint32_t*>(ptr(L.lookup));
   float2* stats = reinterpret_cast<float2*>(ptr(L.stats));
   const bool train = du != nullptr;
   uint16_t* dz = train ? reinterpret_cast<uint16_t*>(ptr(L.dz)) : nullptr;
@@ -492,9 +507,6 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
   const float scale = kLog2e / temperature;
   const int pairs = device_sm_count() / 2;
 
-  gather_kernel<<<static_cast<unsigned>((t + 31) / 32), 256, 0, st>>>(hidden, h, used, t, source, place, count, hc, loss, mass);
-  count_launch();
-  if (int rc = check_launch("distill gather")) return rc;
   CUtensorMap m_w;
   int rc = make_map(&m_w, dt, weight, h, v, h * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
@@ -517,14 +529,13 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
     p.scale = scale;
     p.list = k;
     p.columns = columns;
-    p.source = source;
-    p.starts = starts;
+    p.lookup = lookup;
     p.listed = listed;
     p.stats = stats;
     p.store = train ? 1 : 0;
     rc = dense::launch<false, BF16>(m_h, m_w, train ? m_dz_out : m_h, p, st, "distill_logits");
     if (rc) return rc;
-    merge_kernel<<<static_cast<unsigned>((rows + 7) / 8), kMergeThreads, 0, st>>>(
+    merge_kernel<<<static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows), kMergeThreads, 0, st>>>(
         stats, rows, static_cast<int>(L.tiles), count, static_cast<int>(r0), source, used, logp, rest, k, scale, listed, loss,
         mass, train ? unit : nullptr, shift);
     count_launch();
@@ -532,7 +543,7 @@ int forward(const uint16_t* hidden, int64_t t, int64_t h, const uint16_t* weight
     if (!train) continue;
     const dim3 grid(static_cast<unsigned>((L.pitch / 8 + kScaleThreads * kScaleVecs - 1) / (kScaleThreads * kScaleVecs)),
                     static_cast<unsigned>(rows < 32768 ? rows : 32768), static_cast<unsigned>((rows + 32767) / 32768));
-    scale_kernel<BF16><<<grid, kScaleThreads, 0, st>>>(dz, L.pitch, stats, rows, count, static_cast<int>(r0), source, used,
+    scale_kernel<BF16><<<grid, kScaleThreads, 0, st>>>(dz, L.pitch, stats, rows, count, static_cast<int>(r0), used,
                                                        columns, listed, k, shift);
     count_launch();
     if (int e = check_launch("distill scale")) return e;
@@ -607,18 +618,26 @@ int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint1
   if (!workspace || workspace_bytes < L.total) return sb::fail(SB_EWORKSPACE, "distillation workspace too small");
   cudaStream_t st = sb::as_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  auto prepare = logits_dtype == SB_F32   ? prepare_kernel<float>
-                 : logits_dtype == SB_F16 ? prepare_kernel<__half>
-                                          : prepare_kernel<__nv_bfloat16>;
-  prepare<<<static_cast<unsigned>((t + 3) / 4), 128, 0, st>>>(
-      indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), reinterpret_cast<int*>(ws + L.columns),
-      reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest), reinterpret_cast<int*>(ws + L.used),
-      reinterpret_cast<uint16_t*>(ws + L.starts));
-  sb::count_launch();
-  if (int rc = sb::check_launch("distill prepare")) return rc;
+  const unsigned blocks = static_cast<unsigned>((t + kRowsPerBlock - 1) / kRowsPerBlock);
+  auto lists = [&](auto type) {
+    using T = decltype(type);
+    int* row_blocks = reinterpret_cast<int*>(ws + L.blocks);
+    answered_kernel<T><<<blocks, 256, 0, st>>>(indices, logits, teacher_lse, t, k, v, place, row_blocks);
+    sb::count_launch();
+    prepare_kernel<T><<<blocks, 256, 0, st>>>(
+        hidden, h, indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), row_blocks, place,
+        reinterpret_cast<int*>(ws + L.source), reinterpret_cast<int*>(ws + L.count), reinterpret_cast<uint16_t*>(ws + L.hidden),
+        reinterpret_cast<int*>(ws + L.columns), reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest),
+        reinterpret_cast<int*>(ws + L.used), reinterpret_cast<uint32_t*>(ws + L.lookup), loss, mass);
+    sb::count_launch();
+    return sb::check_launch("distill prepare");
+  };
+  if (int rc = logits_dtype == SB_F32 ? lists(float{}) : logits_dtype == SB_F16 ? lists(__half{}) : lists(__nv_bfloat16{})) {
+    return rc;
+  }
   return dtype == SB_BF16
-             ? forward<true>(hidden, t, h, weight, v, k, temperature, L, ws, loss, mass, du, place, st)
-             : forward<false>(hidden, t, h, weight, v, k, temperature, L, ws, loss, mass, du, place, st);
+             ? forward<true>(t, h, weight, v, k, temperature, L, ws, loss, mass, du, st)
+             : forward<false>(t, h, weight, v, k, temperature, L, ws, loss, mass, du, st);
 }
 
 int sb_distill_backward(const float* du, const int* place, const float* grad, int64_t t, int64_t h, void* dhidden, int dtype,
