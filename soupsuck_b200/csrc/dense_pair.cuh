@@ -263,22 +263,22 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)
   const float m = t == -INFINITY ? 0.0f : ceilf(t * p.scale);
   const uint64_t scale = pair_of(p.scale, p.scale), off = pair_of(kLift - m, kLift - m);
   uint64_t s0 = 0, s1 = 0;
+  const uint32_t swz = static_cast<uint32_t>(lane & 7);
+  // A panel of 64 columns at a time: the first one's store reads the box while the
+  // second one's exponentials are formed.
 #pragma unroll
-  for (int i = 0; i < 64; ++i) {
-    const float2 e = values_of(fma_pair(acc[i], scale, off));
-    acc[i] = pair_of(exp2_fast(e.x), exp2_fast(e.y));
-    if (i & 1) {
-      s1 = add_pair(s1, acc[i]);
-    } else {
-      s0 = add_pair(s0, acc[i]);
+  for (int panel = 0; panel < 2; ++panel) {
+#pragma unroll
+    for (int i = 32 * panel; i < 32 * panel + 32; ++i) {
+      const float2 e = values_of(fma_pair(acc[i], scale, off));
+      acc[i] = pair_of(exp2_fast(e.x), exp2_fast(e.y));
+      if (i & 1) {
+        s1 = add_pair(s1, acc[i]);
+      } else {
+        s0 = add_pair(s0, acc[i]);
+      }
     }
-  }
-  const float2 s = values_of(add_pair(s0, s1));
-  if (valid) p.stats[static_cast<int64_t>(jt) * p.rows_cap + row] = make_float2(m, s.x + s.y);
-  if (p.store) {
-    const uint32_t swz = static_cast<uint32_t>(lane & 7);
-#pragma unroll
-    for (int panel = 0; panel < 2; ++panel) {
+    if (p.store) {
       if (lane == 0) gemm::pair::bulk_wait_read0();
       __syncwarp();
 #pragma unroll
@@ -300,6 +300,8 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)
       }
     }
   }
+  const float2 s = values_of(add_pair(s0, s1));
+  if (valid) p.stats[static_cast<int64_t>(jt) * p.rows_cap + row] = make_float2(m, s.x + s.y);
 }
 
 // ---------------------------------------------------------------- product epilogue
