@@ -62,6 +62,7 @@ struct Params {
   float scale;           // log2(e) / temperature
   int list;              // list length K
   const int* columns;    // [rows of the call, K] listed columns, rising
+  const float* reference;  // [compact rows] exponent that the rows' exponentials share
   const uint32_t* lookup;  // [compact rows, 2 n_tiles] which columns of each 128 are listed (listed_word)
   float* listed;         // [compact rows, K] logits of the listed columns
   float2* stats;         // [2 n_tiles, rows_cap] exponent M and sum of 2^(y - M + 14)
@@ -181,9 +182,20 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// Exponents of the stored exponentials: 2^14 at a 128-column tile's maximum (rounded up
-// to a power of two), so fp16 keeps its 11 bits down to 2^-28 of it.
+// Exponentials are 2^(y - M + 14), y = z log2(e) / tau, with a whole exponent M: the row's
+// reference, a guess of its log-sum-exp and a little more, where the tile's maximum
+// (rounded up) lies from 26 below it to 1 above, else the tile's own maximum.  So fp16
+// holds them without overflow (2^15) and, within a tile, down to 2^-12 of the maximum
+// with an error below 2^-13 of it.  Rows whose tiles all keep the reference need no
+// rescaling afterwards.
 constexpr float kLift = 14.0f;
+constexpr float kBelow = 26.0f, kAbove = 1.0f;
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
 
 // The list entries of one row in one tile of 128 columns: columns of the first three (7
 // bits each), the first one's number in the list (8), how many (2, at most 3), whether
@@ -199,12 +211,12 @@ __device__ __forceinline__ uint32_t listed_word(int first, int n, int c0, int c1
 
 // ---------------------------------------------------------------- logits epilogue
 // acc: this thread's row, columns col0 .. col0 + 127.  Listed columns leave their logit
-// in p.listed and count as absent; the others give the tile's exponent M (the maximum of
-// y = z log2(e) / tau rounded up) and sum of 2^(y - M + 14), which are also stored.
+// in p.listed and count as absent; the others give the tile's exponent M and sum of
+// 2^(y - M + 14), which are also stored.
 template <bool BF16>
 __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)[64], int row, int rows, int col0, int jt,
-                                                uint32_t listed_here, uint8_t* box, const CUtensorMap* tm_out, int row_box,
-                                                int lane) {
+                                                uint32_t listed_here, float reference, uint8_t* box, const CUtensorMap* tm_out,
+                                                int row_box, int lane) {
   const int ncol = p.cols - col0;
   if (ncol < 128) {
 #pragma unroll
@@ -260,7 +272,8 @@ __device__ __forceinline__ void logits_epilogue(const Params& p, uint64_t (&acc)
     top[i & 3] = fmaxf(fmaxf(top[i & 3], y.x), y.y);
   }
   const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  const float m = t == -INFINITY ? 0.0f : ceilf(t * p.scale);
+  float m = t == -INFINITY ? 0.0f : ceilf(t * p.scale);
+  m = m >= reference - kBelow && m <= reference + kAbove ? reference : m;
   const uint64_t scale = pair_of(p.scale, p.scale), off = pair_of(kLift - m, kLift - m);
   uint64_t s0 = 0, s1 = 0;
   const uint32_t swz = static_cast<uint32_t>(lane & 7);
@@ -486,8 +499,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int col0 = u.nt * kTile + half * kHalf;
       const int jt = u.nt * 2 + half;
       uint32_t listed_here = 0;
+      float reference = 0.0f;
       if constexpr (!PRODUCT) {
-        if (row < rows) listed_here = p.lookup[(static_cast<int64_t>(p.row_base) + row) * (2 * p.n_tiles) + jt];
+        if (row < rows) {
+          const int64_t at = static_cast<int64_t>(p.row_base) + row;
+          listed_here = p.lookup[at * (2 * p.n_tiles) + jt];
+          reference = p.reference[at];
+        }
       }
       uint64_t acc[64];
 #pragma unroll
@@ -522,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if constexpr (PRODUCT) {
         product_epilogue(p, acc, col0, box, &tm_out, u.split * units.m_tiles * kTile + row_box, lane);
       } else {
-        logits_epilogue<BF16>(p, acc, row, rows, col0, jt, listed_here, box, &tm_out, row_box, lane);
+        logits_epilogue<BF16>(p, acc, row, rows, col0, jt, listed_here, reference, box, &tm_out, row_box, lane);
       }
     }
     if (lane == 0) bulk_wait_all();

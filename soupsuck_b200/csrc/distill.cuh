@@ -13,16 +13,22 @@
 //
 // Forward.  prepare gathers the answered rows (the others are left out of everything
 // else), sorts each one's list and computes log p.  One tensor-core launch forms the
-// logits tile by tile (dense_pair.cuh): listed ones are written out, the others leave a
-// power-of-two exponent and a sum of exponentials per row and 128 columns, and, where a
-// gradient is wanted, the exponentials themselves in 16 bits [rows, V].  merge joins them
-// per row.  The gradient does not wait for the upstream one, which only scales rows:
-// dz is the stored exponentials times a power of two per tile (exact) with the listed
-// columns written in, du = dz . W on the tensor cores, and the row's remaining factor is
-// applied to the fp32 sums.  Against forming the logits a second time this costs one
-// read and write of the 16-bit array and saves a third of the matrix work.
+// logits tile by tile (dense_pair.cuh): listed ones are written out, the others leave an
+// exponent and a sum of exponentials per row and 128 columns, and, where a gradient is
+// wanted, the exponentials themselves in 16 bits [rows, V].  merge joins them per row.
+// The gradient does not wait for the upstream one, which only scales rows: dz is the
+// stored exponentials with the listed columns written in, du = dz . W on the tensor
+// cores, and the row's remaining factor is applied to the fp32 sums.  A row whose tiles
+// used different exponents, or whose listed columns would overflow beside the others,
+// is first multiplied by powers of two (exact), 4 bytes of traffic per logit that most
+// rows do without: prepare guesses the row's log-sum-exp (from the student's logit of
+// the teacher's best token, as if their probabilities of it were equal) and the tiles
+// use that exponent.  Keeping the exponentials instead of forming the logits a second
+// time saves a third of the matrix work.
 // Backward.  dhidden = upstream * du, rounded once.
 #pragma once
+
+#include <type_traits>
 
 #include "dense_pair.cuh"
 #include "gemm_host.cuh"
@@ -33,6 +39,7 @@ namespace distill {
 constexpr int kMaxList = 256;
 constexpr int kNone = 0x7fffffff;             // an unused entry of a sorted list
 constexpr int64_t kBlockBytes = int64_t(4) << 30;  // 16-bit exponentials of one row block
+constexpr int kMaxRowBlocks = 256;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename T> __device__ __forceinline__ float logit_at(const void* p, int64_t i);
@@ -104,8 +111,9 @@ __global__ void __launch_bounds__(256) answered_kernel(const int64_t* __restrict
 // are used, and which entries each 128-column tile has.  Rows that are not answered get zero
 // loss and mass here.  One warp per row; an entry's place is the number of entries
 // before it (K <= 256).
-template <typename T>
+template <typename T, bool BF16>
 __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict__ hidden, int64_t h,
+                                                      const uint16_t* __restrict__ weight,
                                                       const int64_t* __restrict__ indices, const void* __restrict__ logits,
                                                       const float* __restrict__ lse, int64_t rows, int k, int64_t v,
                                                       float inv_tau, int tiles, const int* __restrict__ blocks,
@@ -113,7 +121,8 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
                                                       int* __restrict__ count, uint16_t* __restrict__ gathered,
                                                       int* __restrict__ columns, float* __restrict__ logp,
                                                       float* __restrict__ rest, int* __restrict__ used,
-                                                      uint32_t* __restrict__ lookup, float* __restrict__ loss,
+                                                      uint32_t* __restrict__ lookup, float* __restrict__ reference,
+                                                      int* __restrict__ uneven, int row_blocks, float* __restrict__ loss,
                                                       float* __restrict__ mass) {
   __shared__ int s_col[kRowsPerBlock][kMaxList];
   __shared__ float s_t[kRowsPerBlock][kMaxList];
@@ -132,6 +141,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
   int at = 0;
   for (int i = 0; i < kRowsPerBlock; ++i) at += s_before[i] + (i < warp ? s_in[i] : 0);
   if (lane == 0 && warp == kRowsPerBlock - 1 && blockIdx.x == gridDim.x - 1) *count = at + s_in[warp];
+  if (blockIdx.x == 0 && threadIdx.x < row_blocks) uneven[threadIdx.x] = 0;
   if (row >= rows) return;
   if (lane == 0) {
     place[row] = in ? at : -1;
@@ -143,14 +153,9 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
     }
   }
   if (!in) return;
-  {
-    const uint4* from = reinterpret_cast<const uint4*>(hidden + row * h);
-    uint4* to = reinterpret_cast<uint4*>(gathered + at * h);
-    for (int64_t i = lane; i < h / 8; i += 32) to[i] = from[i];
-  }
   int* col = s_col[warp];
   float* tv = s_t[warp];
-  int n = 0;
+  int n = 0, best = kNone;  // best: the column of this lane's largest logit
   float top = -INFINITY;
   for (int j = lane; j < k; j += 32) {
     const int64_t c = indices[row * k + j];
@@ -159,10 +164,32 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
     col[j] = used_here ? static_cast<int>(c) : kNone;
     tv[j] = t;
     n += used_here ? 1 : 0;
+    if (used_here && (best == kNone || t > top)) best = static_cast<int>(c);
     top = t == t ? fmaxf(top, t) : INFINITY;  // a NaN makes the row NaN
   }
   for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  const float mine = top;
   top = warp_max(top);
+  best = __shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, best != kNone && mine == top) | 0x80000000u) - 1);
+  if (best == kNone) best = 0;  // (a lane's NaN: any column will do)
+  // The hidden state, and its logit of that column.
+  float dot = 0.0f;
+  {
+    const uint4* from = reinterpret_cast<const uint4*>(hidden + row * h);
+    const uint4* w = reinterpret_cast<const uint4*>(weight + static_cast<int64_t>(best) * h);
+    uint4* to = reinterpret_cast<uint4*>(gathered + at * h);
+    for (int64_t i = lane; i < h / 8; i += 32) {
+      const uint4 a = from[i], b = w[i];
+      to[i] = a;
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = dense::unpack2<BF16>(aw[j]), y = dense::unpack2<BF16>(bw[j]);
+        dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
+      }
+    }
+    dot = warp_sum(dot);
+  }
   __syncwarp();
   // The normaliser: the teacher's, or the list's own.
   float norm;
@@ -190,6 +217,9 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
     const float left = 1.0f - sum;
     rest[at] = !lse || n == v ? 0.0f : (left < 0.0f ? 0.0f : left);
     used[at] = n;
+    // log2 of the student's exponential sum if it gave the teacher's best token the
+    // teacher's probability, and four more for the listed columns' room in 16 bits.
+    reference[at] = ceilf((dot * inv_tau - (top - norm)) * kLog2e) + 4.0f;
   }
   // The tiles' lookups: zeros, then each tile's from its first entry.
   uint32_t* row_lookup = lookup + static_cast<int64_t>(at) * tiles;
@@ -224,12 +254,14 @@ __device__ __forceinline__ float gap(float p, float logp, float q, float logq) {
 }
 
 // Four rows per CTA.  Joins a row's tile statistics and listed logits into its loss and
-// mass, and for the gradient: `shift` so that a tile's exponentials times 2^(M + shift)
-// are dz in the row's unit, `unit` (dz's factor), and the listed columns' dz / unit (over
-// their logits).  The unit is a power of two times the factor all unlisted columns share,
+// mass, and for the gradient: `unit`, dz's factor, and the listed columns' dz / unit,
+// written in among the exponentials.  The unit is a power of two times the factor all
+// unlisted columns share,
 //   b = 2^(R - lse2) - p_rest / S     (R the largest M, S the sum of 2^(y - R)),
 // so only the listed columns' values are rounded anew, and is such that neither passes
-// 2^15 in fp16.
+// 2^15 in fp16.  Rows whose exponentials have to change for that, by 2^(M + shift) in a
+// tile, go to the list `uneven` (its count first); their listed values are kept over
+// their logits for the kernel that does it.
 constexpr int kMergeThreads = 512, kMergeRows = 4;
 constexpr float kLow = -1e9f;  // below every exponent
 
@@ -238,19 +270,27 @@ __device__ __forceinline__ float power(float x) {
   return x > -127.0f ? __int_as_float((static_cast<int>(x) + 127) << 23) : (x == x ? 0.0f : x);
 }
 
+template <bool BF16>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
     const float2* __restrict__ stats, int64_t ld, int tiles, const int* __restrict__ count, int row_base,
     const int* __restrict__ source, const int* __restrict__ used, const float* __restrict__ logp,
     const float* __restrict__ rest, int k, float scale, float* __restrict__ listed, float* __restrict__ loss,
-    float* __restrict__ mass, float* __restrict__ unit, int* __restrict__ shift) {
+    float* __restrict__ mass, const float* __restrict__ reference, const int* __restrict__ columns,
+    uint16_t* __restrict__ dz, int64_t pitch, float* __restrict__ unit, int* __restrict__ shift,
+    int* __restrict__ uneven_count, int* __restrict__ uneven) {
   __shared__ float s_r[kMergeThreads], s_s[kMergeThreads];
+  __shared__ int s_mixed[kMergeRows];
   const int n = *count - row_base;
   const int r = threadIdx.x % kMergeRows, g = threadIdx.x / kMergeRows;
   constexpr int kGroups = kMergeThreads / kMergeRows;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeRows + r;
   if (static_cast<int64_t>(blockIdx.x) * kMergeRows >= n) return;
+  if (threadIdx.x < kMergeRows) s_mixed[threadIdx.x] = 0;
+  __syncthreads();
   float R = kLow, S = 0.0f;
   if (row < n) {
+    const float ref = reference[row_base + row];
+    bool mixed = false;
     // Loads first, several at a time; every factor is a power of two (exact).
     constexpr int kAtOnce = 10;
     for (int j0 = g; j0 < tiles; j0 += kAtOnce * kGroups) {
@@ -261,6 +301,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
         const int64_t j = j0 + i * kGroups;
         t[i] = j < tiles ? stats[j * ld + row] : make_float2(kLow, 0.0f);
         if (t[i].y != 0.0f) top = fmaxf(top, t[i].x);
+        mixed |= t[i].y != 0.0f && t[i].x != ref;
       }
       S *= power(R - top);
 #pragma unroll
@@ -269,6 +310,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
       }
       R = top;
     }
+    if (mixed) s_mixed[r] = 1;
   }
   s_r[threadIdx.x] = R;
   s_s[threadIdx.x] = S;
@@ -332,54 +374,62 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
     e = down - static_cast<int>(R);
     f = ldexpf(a, -down);
   }
-  for (int j = lane; j < m; j += 32) z[j] = z[j] / f;
+  const bool even = S == 0.0f || (s_mixed[warp] == 0 && e == -static_cast<int>(R));
+  const int* row_columns = columns + (row_base + at) * k;
+  for (int j = lane; j < m; j += 32) {
+    const float x = z[j] / f;
+    z[j] = x;
+    if (even) dz[at * pitch + row_columns[j]] = static_cast<uint16_t>(dense::pack2<BF16>(x, 0.0f) & 0xffffu);
+  }
   if (lane == 0) {
     unit[row_base + at] = f;
     shift[row_base + at] = e;
+    if (!even) uneven[atomicAdd(uneven_count, 1)] = static_cast<int>(at);
   }
 }
 
-// dz of one row's segment in place: each tile's exponentials times 2^(M + shift), then
-// the listed columns.
+// The uneven rows' dz in place, a segment of a row at a time: each tile's exponentials
+// times 2^(M + shift), then the listed columns.
 constexpr int kScaleThreads = 256, kScaleVecs = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(kScaleThreads) scale_kernel(
-    uint16_t* __restrict__ dz, int64_t pitch, const float2* __restrict__ stats, int64_t ld, const int* __restrict__ count,
-    int row_base, const int* __restrict__ used, const int* __restrict__ columns, const float* __restrict__ listed, int k, const int* __restrict__ shift) {
-  const int64_t row = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 32768;
-  if (row >= *count - row_base || row >= ld) return;
-  const int e = shift[row_base + row];
-  uint16_t* line = dz + row * pitch;
-  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * kScaleThreads * kScaleVecs;
+    uint16_t* __restrict__ dz, int64_t pitch, const float2* __restrict__ stats, int64_t ld,
+    const int* __restrict__ uneven_count, const int* __restrict__ uneven, int row_base, const int* __restrict__ used,
+    const int* __restrict__ columns, const float* __restrict__ listed, int k, const int* __restrict__ shift) {
+  constexpr int kSegment = kScaleThreads * kScaleVecs;  // vectors
+  const int segments = static_cast<int>((pitch / 8 + kSegment - 1) / kSegment);
+  const int64_t items = static_cast<int64_t>(*uneven_count) * segments;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = uneven[item / segments];
+    const int e = shift[row_base + row];
+    uint16_t* line = dz + row * pitch;
+    const int64_t v0 = item % segments * kSegment;
 #pragma unroll
-  for (int i = 0; i < kScaleVecs; ++i) {
-    const int64_t vec = v0 + i * kScaleThreads + threadIdx.x;
-    if (vec * 8 >= pitch) break;
-    const float2 t = stats[(vec >> 4) * ld + row];
-    const int by = static_cast<int>(t.x) + e;
-    if (by == 0 || t.y == 0.0f) continue;
-    const float f = exp2f(static_cast<float>(by));
-    uint4* at = reinterpret_cast<uint4*>(line) + vec;
-    uint4 w = *at;
-    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+    for (int i = 0; i < kScaleVecs; ++i) {
+      const int64_t vec = v0 + i * kScaleThreads + threadIdx.x;
+      if (vec * 8 >= pitch) break;
+      const float2 t = stats[(vec >> 4) * ld + row];
+      const int by = static_cast<int>(t.x) + e;
+      if (by == 0 || t.y == 0.0f) continue;
+      const float f = exp2f(static_cast<float>(by));
+      uint4* at = reinterpret_cast<uint4*>(line) + vec;
+      uint4 w = *at;
+      uint32_t* x = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (BF16) {
-        x[j] = dense::pack2<true>(__uint_as_float(x[j] << 16) * f, __uint_as_float(x[j] & 0xffff0000u) * f);
-      } else {
-        const float2 y = __half22float2(*reinterpret_cast<__half2*>(&x[j]));
-        x[j] = dense::pack2<false>(y.x * f, y.y * f);
+      for (int j = 0; j < 4; ++j) {
+        const float2 y = dense::unpack2<BF16>(x[j]);
+        x[j] = dense::pack2<BF16>(y.x * f, y.y * f);
       }
+      *at = w;
     }
-    *at = w;
-  }
-  __syncthreads();
-  const int64_t c0 = v0 * 8, c1 = c0 + kScaleThreads * kScaleVecs * 8;
-  const int n = used[row_base + row];
-  for (int j = threadIdx.x; j < n; j += kScaleThreads) {
-    const int c = columns[(row_base + row) * k + j];
-    if (c >= c0 && c < c1) {
-      line[c] = static_cast<uint16_t>(dense::pack2<BF16>(listed[(row_base + row) * k + j], 0.0f) & 0xffffu);
+    __syncthreads();
+    const int64_t c0 = v0 * 8, c1 = c0 + kSegment * 8;
+    const int n = used[row_base + row];
+    for (int j = threadIdx.x; j < n; j += kScaleThreads) {
+      const int c = columns[(row_base + row) * k + j];
+      if (c >= c0 && c < c1) {
+        line[c] = static_cast<uint16_t>(dense::pack2<BF16>(listed[(row_base + row) * k + j], 0.0f) & 0xffffu);
+      }
     }
   }
 }
@@ -432,7 +482,7 @@ __global__ void __launch_bounds__(256) backward_kernel(const float* __restrict__
 struct Layout {
   int64_t tiles, pitch, cap, room;
   int n_tiles, out_tiles, k_blocks;
-  size_t columns, logp, listed, rest, used, source, blocks, count, unit, shift, hidden, lookup, stats, dz, parts, total;
+  size_t columns, logp, listed, rest, used, source, blocks, count, unit, shift, reference, uneven, uneven_counts, hidden, lookup, stats, dz, parts, total;
 };
 
 inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
@@ -443,7 +493,8 @@ inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
   L.cap = t;
   if (train) {
     int64_t rows = kBlockBytes / (L.pitch * 2) / dense::kTile * dense::kTile;
-    if (rows < dense::kTile) rows = dense::kTile;
+    const int64_t least = ((t + kMaxRowBlocks - 1) / kMaxRowBlocks + dense::kTile - 1) / dense::kTile * dense::kTile;
+    if (rows < least) rows = least;
     if (rows < t) L.cap = rows;
   }
   L.out_tiles = static_cast<int>((h + dense::kTile - 1) / dense::kTile);
@@ -464,6 +515,9 @@ inline Layout layout(int64_t t, int64_t h, int64_t v, int k, bool train) {
   L.count = take(16);
   L.unit = take(t * 4);
   L.shift = take(t * 4);
+  L.reference = take(t * 4);
+  L.uneven = take(L.cap * 4);
+  L.uneven_counts = take(kMaxRowBlocks * 4);
   L.hidden = take(t * h * 2);
   L.lookup = take(L.tiles * t * 4);
   L.stats = take(L.tiles * L.cap * 8);
@@ -497,6 +551,8 @@ int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, floa
   int* count = reinterpret_cast<int*>(ptr(L.count));
   float* unit = reinterpret_cast<float*>(ptr(L.unit));
   int* shift = reinterpret_cast<int*>(ptr(L.shift));
+  const float* reference = reinterpret_cast<const float*>(ptr(L.reference));
+  int* uneven = reinterpret_cast<int*>(ptr(L.uneven));
   uint16_t* hc = reinterpret_cast<uint16_t*>(ptr(L.hidden));
   uint32_t* lookup = reinterpret_cast<uint32_t*>(ptr(L.lookup));
   float2* stats = reinterpret_cast<float2*>(ptr(L.stats));
@@ -530,21 +586,21 @@ int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, floa
     p.list = k;
     p.columns = columns;
     p.lookup = lookup;
+    p.reference = reference;
     p.listed = listed;
     p.stats = stats;
     p.store = train ? 1 : 0;
     rc = dense::launch<false, BF16>(m_h, m_w, train ? m_dz_out : m_h, p, st, "distill_logits");
     if (rc) return rc;
-    merge_kernel<<<static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows), kMergeThreads, 0, st>>>(
+    int* uneven_count = reinterpret_cast<int*>(ptr(L.uneven_counts)) + r0 / L.cap;
+    merge_kernel<BF16><<<static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows), kMergeThreads, 0, st>>>(
         stats, rows, static_cast<int>(L.tiles), count, static_cast<int>(r0), source, used, logp, rest, k, scale, listed, loss,
-        mass, train ? unit : nullptr, shift);
+        mass, reference, columns, dz, L.pitch, train ? unit : nullptr, shift, uneven_count, uneven);
     count_launch();
     if (int e = check_launch("distill merge")) return e;
     if (!train) continue;
-    const dim3 grid(static_cast<unsigned>((L.pitch / 8 + kScaleThreads * kScaleVecs - 1) / (kScaleThreads * kScaleVecs)),
-                    static_cast<unsigned>(rows < 32768 ? rows : 32768), static_cast<unsigned>((rows + 32767) / 32768));
-    scale_kernel<BF16><<<grid, kScaleThreads, 0, st>>>(dz, L.pitch, stats, rows, count, static_cast<int>(r0), used,
-                                                       columns, listed, k, shift);
+    scale_kernel<BF16><<<static_cast<unsigned>(device_sm_count() * 8), kScaleThreads, 0, st>>>(
+        dz, L.pitch, stats, rows, uneven_count, uneven, static_cast<int>(r0), used, columns, listed, k, shift);
     count_launch();
     if (int e = check_launch("distill scale")) return e;
     rc = make_map(&m_dz, dt, dz, L.pitch, rows, L.pitch * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -619,22 +675,25 @@ int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint1
   cudaStream_t st = sb::as_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const unsigned blocks = static_cast<unsigned>((t + kRowsPerBlock - 1) / kRowsPerBlock);
-  auto lists = [&](auto type) {
+  const int row_blocks = static_cast<int>((t + L.cap - 1) / L.cap);
+  auto lists = [&](auto type, auto half) {
     using T = decltype(type);
-    int* row_blocks = reinterpret_cast<int*>(ws + L.blocks);
-    answered_kernel<T><<<blocks, 256, 0, st>>>(indices, logits, teacher_lse, t, k, v, place, row_blocks);
+    int* answered = reinterpret_cast<int*>(ws + L.blocks);
+    answered_kernel<T><<<blocks, 256, 0, st>>>(indices, logits, teacher_lse, t, k, v, place, answered);
     sb::count_launch();
-    prepare_kernel<T><<<blocks, 256, 0, st>>>(
-        hidden, h, indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), row_blocks, place,
+    prepare_kernel<T, decltype(half)::value><<<blocks, 256, 0, st>>>(
+        hidden, h, weight, indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), answered, place,
         reinterpret_cast<int*>(ws + L.source), reinterpret_cast<int*>(ws + L.count), reinterpret_cast<uint16_t*>(ws + L.hidden),
         reinterpret_cast<int*>(ws + L.columns), reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest),
-        reinterpret_cast<int*>(ws + L.used), reinterpret_cast<uint32_t*>(ws + L.lookup), loss, mass);
+        reinterpret_cast<int*>(ws + L.used), reinterpret_cast<uint32_t*>(ws + L.lookup),
+        reinterpret_cast<float*>(ws + L.reference), reinterpret_cast<int*>(ws + L.uneven_counts), row_blocks, loss, mass);
     sb::count_launch();
     return sb::check_launch("distill prepare");
   };
-  if (int rc = logits_dtype == SB_F32 ? lists(float{}) : logits_dtype == SB_F16 ? lists(__half{}) : lists(__nv_bfloat16{})) {
-    return rc;
-  }
+  auto typed = [&](auto half) {
+    return logits_dtype == SB_F32 ? lists(float{}, half) : logits_dtype == SB_F16 ? lists(__half{}, half) : lists(__nv_bfloat16{}, half);
+  };
+  if (int rc = dtype == SB_BF16 ? typed(std::true_type{}) : typed(std::false_type{})) return rc;
   return dtype == SB_BF16
              ? forward<true>(t, h, weight, v, k, temperature, L, ws, loss, mass, du, st)
              : forward<false>(t, h, weight, v, k, temperature, L, ws, loss, mass, du, st);
