@@ -26,6 +26,8 @@
 
 #include <cuda_bf16.h>
 
+#include <mutex>
+
 #include "gemm_pair.cuh"
 
 namespace sb {
@@ -105,7 +107,8 @@ struct Unit {
 
 // Logits: whole-K tiles, rows fastest (the pairs of a wave share columns of W).
 // Product: (split, tile) with columns fastest, so the pairs of a wave walk the same
-// k range together and share their operands in L2.
+// k-blocks together and share their operands in L2.  Split s takes every splits-th block,
+// from the last one down: each begins with what the logits launch left in L2.
 template <bool PRODUCT>
 struct Units {
   int m_tiles, tiles, splits, cursor, end, stride;
@@ -124,8 +127,8 @@ struct Units {
       const int t = cursor % tiles;
       u.m0 = t / p.n_tiles * kTile;
       u.nt = t % p.n_tiles;
-      u.k0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * u.split / splits);
-      u.k1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (u.split + 1) / splits);
+      u.k0 = 0;
+      u.k1 = (p.k_blocks - u.split + splits - 1) / splits;
     } else {
       u.split = 0;
       u.m0 = cursor % m_tiles * kTile;
@@ -410,12 +413,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint8_t* a_s = smem + s * kStageBytes;
             uint8_t* b_s = a_s + kOperandBytes;
             if (leader) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
-            tma_load_2d_pair(a_s, &tm_a, leader_full + 8u * s, kb * kBK, arow);
+            const int k = PRODUCT ? ((u.k1 - 1 - kb) * splits + u.split) * kBK : kb * kBK;
+            tma_load_2d_pair(a_s, &tm_a, leader_full + 8u * s, k, arow);
             if constexpr (PRODUCT) {
-              tma_load_2d_pair(b_s, &tm_b, leader_full + 8u * s, bcol, kb * kBK);
-              tma_load_2d_pair(b_s + kOperandBytes / 2, &tm_b, leader_full + 8u * s, bcol + 64, kb * kBK);
+              tma_load_2d_pair(b_s, &tm_b, leader_full + 8u * s, bcol, k);
+              tma_load_2d_pair(b_s + kOperandBytes / 2, &tm_b, leader_full + 8u * s, bcol + 64, k);
             } else {
-              tma_load_2d_pair(b_s, &tm_b, leader_full + 8u * s, kb * kBK, bcol);
+              tma_load_2d_pair(b_s, &tm_b, leader_full + 8u * s, k, bcol);
             }
           }
         }
@@ -559,8 +563,18 @@ template <bool PRODUCT, bool BF16>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Params& p, cudaStream_t st,
            const char* name) {
   auto kern = dense_kernel<PRODUCT, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return fail(SB_ECUDA, std::string(name) + " smem attribute: " + cudaGetErrorString(e));
+  static std::mutex mu;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+      if (e != cudaSuccess) return fail(SB_ECUDA, std::string(name) + " smem attribute: " + cudaGetErrorString(e));
+      if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+  }
   kern<<<device_sm_count() / 2 * 2, kThreads, kSmemBytes, st>>>(a, b, out, p);
   count_launch();
   return check_launch(name);

@@ -23,6 +23,12 @@ from .. import _lib
 from .._spec import BRAIN, HALF, LONG, SINGLE, WIDE_FLOATS, Number, Operand, admit, refuse
 
 MAX_K = 256
+_HIDDEN = Operand(HALF, BRAIN, ndim=2, layout=None)
+_WEIGHT = {dtype: Operand(dtype, ndim=2, layout=None, frozen=True) for dtype in (HALF, BRAIN)}
+_INDICES = Operand(LONG, ndim=2, layout=None)
+_LOGITS = Operand(*WIDE_FLOATS, ndim=2, layout=None, frozen=True)
+_LSE = Operand(SINGLE, ndim=1, layout=None, frozen=True, optional=True)
+_TEMPERATURE = Number()
 
 
 def _operand(t, width):
@@ -56,7 +62,7 @@ class _HeadDistillation(torch.autograd.Function):
                       _lib.wide_dtype_code(w.dtype), indices.data_ptr(), logits.data_ptr(),
                       _lib.wide_dtype_code(logits.dtype), listed, _lib.ptr(lse), temperature, loss.data_ptr(),
                       mass.data_ptr(), _lib.ptr(du), place.data_ptr(), scratch.data_ptr(), nbytes,
-                      _lib.stream_of(dev))
+                      _lib.raw_stream(dev))
         if gradient:
             ctx.save_for_backward(du, place)
         ctx.meta = (hidden.dtype, width)
@@ -74,10 +80,10 @@ class _HeadDistillation(torch.autograd.Function):
         rows, padded = du.shape
         dx = torch.empty((rows, padded), device=du.device, dtype=dtype)
         if rows:
-            with torch.cuda.device(du.device):
-                g = grad_loss.to(SINGLE).contiguous()
+            with _lib.on_device(du.device):
+                g = grad_loss.contiguous()
                 _lib.call("sb_distill_backward", du.data_ptr(), place.data_ptr(), g.data_ptr(), rows, padded,
-                          dx.data_ptr(), _lib.wide_dtype_code(dtype), _lib.stream_of(du.device))
+                          dx.data_ptr(), _lib.wide_dtype_code(dtype), _lib.raw_stream(du.device))
         return (dx[:, :width],) + (None,) * 6
 
 
@@ -106,12 +112,9 @@ def fused_linear_distillation(hidden, weight, indices, logits, teacher_lse=None,
     within a row give an unspecified loss."""
     entry = "fused_linear_distillation"
     device = hidden.device if isinstance(hidden, torch.Tensor) else None
-    admit(entry, device, hidden=(hidden, Operand(HALF, BRAIN, ndim=2, layout=None)))
-    admit(entry, device, weight=(weight, Operand(hidden.dtype, ndim=2, layout=None, frozen=True)),
-          indices=(indices, Operand(LONG, ndim=2, layout=None)),
-          logits=(logits, Operand(*WIDE_FLOATS, ndim=2, layout=None, frozen=True)),
-          teacher_lse=(teacher_lse, Operand(SINGLE, ndim=1, layout=None, frozen=True, optional=True)),
-          temperature=(temperature, Number()))
+    admit(entry, device, hidden=(hidden, _HIDDEN))
+    admit(entry, device, weight=(weight, _WEIGHT[hidden.dtype]), indices=(indices, _INDICES), logits=(logits, _LOGITS),
+          teacher_lse=(teacher_lse, _LSE), temperature=(temperature, _TEMPERATURE))
     rows, vocab = hidden.shape[0], weight.shape[0]
     if vocab == 0 or weight.shape[1] == 0:
         refuse(entry, f"weight {tuple(weight.shape)} has an empty vocabulary or hidden size")
@@ -124,7 +127,7 @@ def fused_linear_distillation(hidden, weight, indices, logits, teacher_lse=None,
         refuse(entry, f"indices list {indices.shape[1]} tokens per row; between 1 and {MAX_K} are taken")
     if not temperature > 0:
         refuse(entry, f"temperature is {temperature!r}; a positive value is required")
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         if validate and rows:
             check_lists(indices.contiguous(), vocab)
         gradient = hidden.requires_grad and torch.is_grad_enabled()
