@@ -385,6 +385,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  // Launched with programmatic stream serialisation (launch_after): the set-up above
+  // overlaps the previous kernel; its results are read from here on.
+  grid_dependency_wait();
+  launch_dependents();
   const int rows = block_rows(p);
   const int splits = PRODUCT && rows > 0 ? product_splits(rows, p.cols, p.k_blocks, pairs, p.room) : 1;
   const uint32_t leader_full = map_to_rank(smem_addr(full), 0);
@@ -559,6 +563,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
+// A launch that may begin while the previous kernel of the stream ends; the kernel waits
+// for it (grid_dependency_wait) before it touches memory.  Every kernel launched this way
+// waits, so a kernel's results are complete for all later ones, not only the next.
+template <typename... P, typename... A>
+int launch_after(const char* name, void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e != cudaSuccess) return fail(SB_ECUDA, std::string(name) + ": " + cudaGetErrorString(e));
+  count_launch();
+  return check_launch(name);
+}
+
 template <bool PRODUCT, bool BF16>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const Params& p, cudaStream_t st,
            const char* name) {
@@ -575,9 +600,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, c
       if (dev >= 0 && dev < 64) configured[dev] = true;
     }
   }
-  kern<<<device_sm_count() / 2 * 2, kThreads, kSmemBytes, st>>>(a, b, out, p);
-  count_launch();
-  return check_launch(name);
+  return launch_after(name, kern, device_sm_count() / 2 * 2, kThreads, kSmemBytes, st, a, b, out, p);
 }
 
 }  // namespace dense

@@ -127,6 +127,8 @@ __global__ void __launch_bounds__(256) prepare_kernel(const uint16_t* __restrict
   __shared__ int s_col[kRowsPerBlock][kMaxList];
   __shared__ float s_t[kRowsPerBlock][kMaxList];
   __shared__ int s_before[kRowsPerBlock], s_in[kRowsPerBlock];
+  grid_dependency_wait();
+  launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + warp;
   int before = 0;
@@ -280,6 +282,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
     int* __restrict__ uneven_count, int* __restrict__ uneven) {
   __shared__ float s_r[kMergeThreads], s_s[kMergeThreads];
   __shared__ int s_mixed[kMergeRows];
+  grid_dependency_wait();
+  launch_dependents();
   const int n = *count - row_base;
   const int r = threadIdx.x % kMergeRows, g = threadIdx.x / kMergeRows;
   constexpr int kGroups = kMergeThreads / kMergeRows;
@@ -397,6 +401,8 @@ __global__ void __launch_bounds__(kScaleThreads) scale_kernel(
     const int* __restrict__ uneven_count, const int* __restrict__ uneven, int row_base, const int* __restrict__ used,
     const int* __restrict__ columns, const float* __restrict__ listed, int k, const int* __restrict__ shift) {
   constexpr int kSegment = kScaleThreads * kScaleVecs;  // vectors
+  grid_dependency_wait();
+  launch_dependents();
   const int segments = static_cast<int>((pitch / 8 + kSegment - 1) / kSegment);
   const int64_t items = static_cast<int64_t>(*uneven_count) * segments;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
@@ -438,6 +444,8 @@ __global__ void __launch_bounds__(kScaleThreads) scale_kernel(
 __global__ void __launch_bounds__(256) sum_kernel(const float* __restrict__ parts, int64_t h, int k_blocks, int pairs,
                                                   int64_t room, const int* __restrict__ count, int row_base, int rows_cap,
                                                   const float* __restrict__ unit, float inv_tau, float* __restrict__ du) {
+  grid_dependency_wait();
+  launch_dependents();
   const int left = *count - row_base;
   const int rows = left < rows_cap ? left : rows_cap;
   if (rows <= 0) return;
@@ -593,16 +601,16 @@ int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, floa
     rc = dense::launch<false, BF16>(m_h, m_w, train ? m_dz_out : m_h, p, st, "distill_logits");
     if (rc) return rc;
     int* uneven_count = reinterpret_cast<int*>(ptr(L.uneven_counts)) + r0 / L.cap;
-    merge_kernel<BF16><<<static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows), kMergeThreads, 0, st>>>(
-        stats, rows, static_cast<int>(L.tiles), count, static_cast<int>(r0), source, used, logp, rest, k, scale, listed, loss,
-        mass, reference, columns, dz, L.pitch, train ? unit : nullptr, shift, uneven_count, uneven);
-    count_launch();
-    if (int e = check_launch("distill merge")) return e;
+    rc = dense::launch_after("distill_merge", merge_kernel<BF16>, static_cast<unsigned>((rows + kMergeRows - 1) / kMergeRows),
+                             kMergeThreads, 0, st, stats, rows, static_cast<int>(L.tiles), count, static_cast<int>(r0), source,
+                             used, logp, rest, k, scale, listed, loss, mass, reference, columns, dz, L.pitch,
+                             train ? unit : nullptr, shift, uneven_count, uneven);
+    if (rc) return rc;
     if (!train) continue;
-    scale_kernel<BF16><<<static_cast<unsigned>(device_sm_count() * 8), kScaleThreads, 0, st>>>(
-        dz, L.pitch, stats, rows, uneven_count, uneven, static_cast<int>(r0), used, columns, listed, k, shift);
-    count_launch();
-    if (int e = check_launch("distill scale")) return e;
+    rc = dense::launch_after("distill_scale", scale_kernel<BF16>, static_cast<unsigned>(device_sm_count() * 8), kScaleThreads, 0,
+                             st, dz, L.pitch, stats, rows, uneven_count, uneven, static_cast<int>(r0), used, columns, listed, k,
+                             shift);
+    if (rc) return rc;
     rc = make_map(&m_dz, dt, dz, L.pitch, rows, L.pitch * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = make_map(&m_wn, dt, weight, h, v, h * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) {
@@ -621,10 +629,10 @@ int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, floa
     d.room = L.room;
     rc = dense::launch<true, BF16>(m_dz, m_wn, m_parts, d, st, "distill_product");
     if (rc) return rc;
-    sum_kernel<<<static_cast<unsigned>(device_sm_count() * 4), 256, 0, st>>>(
-        parts, h, L.k_blocks, pairs, L.room, count, static_cast<int>(r0), static_cast<int>(rows), unit, 1.0f / temperature, du);
-    count_launch();
-    if (int e = check_launch("distill sum")) return e;
+    rc = dense::launch_after("distill_sum", sum_kernel, static_cast<unsigned>(device_sm_count() * 4), 256, 0, st, parts, h,
+                             L.k_blocks, pairs, L.room, count, static_cast<int>(r0), static_cast<int>(rows), unit,
+                             1.0f / temperature, du);
+    if (rc) return rc;
   }
   return SB_OK;
 }
@@ -681,14 +689,14 @@ int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint1
     int* answered = reinterpret_cast<int*>(ws + L.blocks);
     answered_kernel<T><<<blocks, 256, 0, st>>>(indices, logits, teacher_lse, t, k, v, place, answered);
     sb::count_launch();
-    prepare_kernel<T, decltype(half)::value><<<blocks, 256, 0, st>>>(
-        hidden, h, weight, indices, logits, teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), answered, place,
+    if (int rc = sb::check_launch("distill_answered")) return rc;
+    return sb::dense::launch_after(
+        "distill_prepare", prepare_kernel<T, decltype(half)::value>, blocks, 256, 0, st, hidden, h, weight, indices, logits,
+        teacher_lse, t, k, v, 1.0f / temperature, static_cast<int>(L.tiles), answered, place,
         reinterpret_cast<int*>(ws + L.source), reinterpret_cast<int*>(ws + L.count), reinterpret_cast<uint16_t*>(ws + L.hidden),
         reinterpret_cast<int*>(ws + L.columns), reinterpret_cast<float*>(ws + L.logp), reinterpret_cast<float*>(ws + L.rest),
         reinterpret_cast<int*>(ws + L.used), reinterpret_cast<uint32_t*>(ws + L.lookup),
         reinterpret_cast<float*>(ws + L.reference), reinterpret_cast<int*>(ws + L.uneven_counts), row_blocks, loss, mass);
-    sb::count_launch();
-    return sb::check_launch("distill prepare");
   };
   auto typed = [&](auto half) {
     return logits_dtype == SB_F32 ? lists(float{}, half) : logits_dtype == SB_F16 ? lists(__half{}, half) : lists(__nv_bfloat16{}, half);
