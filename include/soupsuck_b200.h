@@ -356,6 +356,11 @@ int sb_distill_forward(const uint16_t* hidden, int64_t t, int64_t h, const uint1
 int sb_distill_backward(const float* du, const int* place, const float* grad, int64_t t, int64_t h, void* dhidden,
                         int dtype, void* stream);
 int sb_distill_check(const int64_t* indices, int64_t t, int k, int64_t v, int64_t* faults, void* stream);
+/* sb_pad_rows: 16-bit rows [rows, h] (row stride in elements, 2-byte alignment) copied to
+ *   [rows, width] with zero columns behind, 16-byte aligned: the layout sb_distill_forward
+ *   takes. */
+int sb_pad_rows(const uint16_t* in, int64_t rows, int64_t h, int64_t row_stride, int64_t width, uint16_t* out,
+                void* stream);
 
 /* sb_verify_drafts: target probabilities [batch, drafts + 1, v] and draft probabilities
  *   [batch, drafts, v] (or NULL: the drafts were chosen, their distribution is one-hot) of

@@ -89,6 +89,7 @@ SIGNATURES = {
                                   _P, _SZ, _P]),
     "sb_distill_backward": (_I32, [_P, _P, _P, _I64, _I64, _P, _I32, _P]),
     "sb_distill_check": (_I32, [_P, _I64, _I32, _I64, _P, _P]),
+    "sb_pad_rows": (_I32, [_P, _I64, _I64, _I64, _I64, _P, _P]),
     "sb_verify_drafts": (_I32, [_P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _P, _P, _P, _I64,
                                 _P, _P, _P, _P]),
 }

@@ -33,11 +33,13 @@ _TEMPERATURE = Number()
 
 def _operand(t, width):
     """t [rows, h] contiguous, 16-byte aligned, with zero columns up to `width`."""
-    if t.shape[1] == width:
+    if t.shape[1] == width and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
-        return t if t.data_ptr() % 16 == 0 else t.clone()
-    out = torch.zeros((t.shape[0], width), dtype=t.dtype, device=t.device)
-    out[:, :t.shape[1]] = t
+    out = torch.empty((t.shape[0], width), dtype=t.dtype, device=t.device)
+    _lib.call("sb_pad_rows", t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), width, out.data_ptr(),
+              _lib.raw_stream(t.device))
     return out
 
 
