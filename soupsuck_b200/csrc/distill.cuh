@@ -41,6 +41,7 @@ constexpr int kNone = 0x7fffffff;             // an unused entry of a sorted lis
 constexpr int64_t kBlockBytes = int64_t(4) << 30;  // 16-bit exponentials of one row block
 constexpr int kMaxRowBlocks = 256;
 constexpr int kFixes = 4;
+constexpr int kPadAtOnce = 4;  // vectors of a thread in flight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename T> __device__ __forceinline__ float logit_at(const void* p, int64_t i);
@@ -66,33 +67,47 @@ __device__ __forceinline__ float warp_max(float x) {
 // the two aligned 16-byte words around them; words past the last element are not read.
 __global__ void __launch_bounds__(256) pad_kernel(const uint16_t* __restrict__ in, int64_t rows, int64_t h, int64_t pitch,
                                                   int64_t width, uint16_t* __restrict__ out) {
-  const int per_row = static_cast<int>(width / 8);
+  const uint32_t per_row = static_cast<uint32_t>(width / 8);
   const uint16_t* end = in + (rows - 1) * pitch + h;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows * per_row;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = i / per_row;
-    const int64_t col = (i - row * per_row) * 8;
-    const uint16_t* from = in + row * pitch + col;
-    const int have = h - col < 8 ? static_cast<int>(h - col) : 8;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(from) & 15) / 2;
-    if (have == 8 && from - off >= in && from - off + 16 <= end) {
-      const uint4* a = reinterpret_cast<const uint4*>(from - off);
-      const uint4 x = __ldcs(a), y = __ldcs(a + 1);
-      const uint32_t all[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  const int64_t vecs = rows * per_row, step = static_cast<int64_t>(gridDim.x) * 256 * kPadAtOnce;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 256 * kPadAtOnce + threadIdx.x; first < vecs; first += step) {
+    const uint16_t* from[kPadAtOnce];
+    int have[kPadAtOnce];
+    uint4 x[kPadAtOnce], y[kPadAtOnce];
 #pragma unroll
-      for (int o = 0; o < 8; ++o) {
-        if (o == off) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = o & 1 ? __funnelshift_r(all[j + o / 2], all[j + o / 2 + 1 < 8 ? j + o / 2 + 1 : 7], 16) : all[j + o / 2];
-          }
-        }
+    for (int u = 0; u < kPadAtOnce; ++u) {
+      const int64_t i = first + u * 256;
+      const int64_t row = vecs <= 0xffffffffll ? static_cast<uint32_t>(i) / per_row : i / per_row;
+      const int64_t col = (i - row * per_row) * 8;
+      from[u] = in + row * pitch + col;
+      have[u] = i < vecs ? (h - col < 8 ? static_cast<int>(h - col) : 8) : 0;
+      const uint16_t* base = from[u] - static_cast<int>(reinterpret_cast<uintptr_t>(from[u]) & 15) / 2;
+      if (have[u] == 8 && base >= in && base + 16 <= end) {
+        x[u] = __ldg(reinterpret_cast<const uint4*>(base));
+        y[u] = __ldg(reinterpret_cast<const uint4*>(base) + 1);
+      } else {
+        have[u] |= 16;
       }
-    } else {
-      for (int j = 0; j < have; ++j) w[j / 2] |= static_cast<uint32_t>(from[j]) << (16 * (j & 1));
     }
-    reinterpret_cast<uint4*>(out)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+    for (int u = 0; u < kPadAtOnce; ++u) {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      if (have[u] < 16) {
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(from[u]) & 15) / 2;
+        // Words off / 2 .. off / 2 + 4 of the eight, shifted by half a word where off is odd.
+        uint32_t a[5] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x};
+        if (off & 2) { a[0] = a[1]; a[1] = a[2]; a[2] = a[3]; a[3] = a[4]; a[4] = y[u].y; }
+        if (off & 4) {
+          const uint32_t next = off & 2 ? y[u].z : y[u].y, then = off & 2 ? y[u].w : y[u].z;
+          a[0] = a[2]; a[1] = a[3]; a[2] = a[4]; a[3] = next; a[4] = then;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = off & 1 ? __funnelshift_r(a[j], a[j + 1], 16) : a[j];
+      } else {
+        for (int j = 0; j < (have[u] & 15); ++j) w[j / 2] |= static_cast<uint32_t>(from[u][j]) << (16 * (j & 1));
+      }
+      if (first + u * 256 < vecs) reinterpret_cast<uint4*>(out)[first + u * 256] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -739,7 +754,7 @@ int sb_pad_rows(const uint16_t* in, int64_t rows, int64_t h, int64_t row_stride,
   SB_REQUIRE(in && out, "NULL pointer argument");
   SB_REQUIRE(row_stride >= 0 && sb::aligned(in, 2) && sb::aligned(out, 16), "bad stride or alignment");
   cudaStream_t st = sb::as_stream(stream);
-  const int64_t blocks = (rows * (width / 8) + 255) / 256, most = static_cast<int64_t>(sb::device_sm_count()) * 16;
+  const int64_t blocks = (rows * (width / 8) + 256 * sb::distill::kPadAtOnce - 1) / (256 * sb::distill::kPadAtOnce), most = static_cast<int64_t>(sb::device_sm_count()) * 16;
   sb::distill::pad_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(in, rows, h, row_stride, width, out);
   sb::count_launch();
   return sb::check_launch("pad_rows");

@@ -77,6 +77,9 @@ template <> struct Kind<float> {
   static __device__ __forceinline__ float top(const uint4& v) {
     return fmaxf(fmaxf(value(v, 0), value(v, 1)), fmaxf(value(v, 2), value(v, 3)));
   }
+  static __device__ __forceinline__ float top4(const uint4 (&q)[kVecs]) {
+    return fmaxf(fmaxf(top(q[0]), top(q[1])), fmaxf(top(q[2]), top(q[3])));
+  }
   static __device__ __forceinline__ Limit limit(float t) { return Limit{t}; }
   static __device__ __forceinline__ bool above(const uint4& v, Limit l) {
     return !(value(v, 0) <= l.t && value(v, 1) <= l.t && value(v, 2) <= l.t && value(v, 3) <= l.t);
@@ -119,6 +122,11 @@ template <> struct Kind<__half> : Kind16<__half, __half2> {
     const float2 f = __half22float2(top2(v));
     return fmaxf(f.x, f.y);
   }
+  // (Of the numbers: a NaN is left out.)
+  static __device__ __forceinline__ float top4(const uint4 (&q)[kVecs]) {
+    const float2 f = __half22float2(__hmax2(__hmax2(top2(q[0]), top2(q[1])), __hmax2(top2(q[2]), top2(q[3]))));
+    return fmaxf(f.x, f.y);
+  }
   // Every threshold is a value of the type (or NaN), so the rounding is exact.
   static __device__ __forceinline__ Limit limit(float t) { return limit_of(__float2half_rn(t)); }
   static __device__ __forceinline__ bool above(const uint4& v, Limit l) { return !__hble2(top2(v), l.t); }
@@ -147,6 +155,11 @@ template <> struct Kind<__nv_bfloat16> : Kind16<__nv_bfloat16, __nv_bfloat162> {
   }
   static __device__ __forceinline__ float top(const uint4& v) {
     const float2 f = __bfloat1622float2(top2(v));
+    return fmaxf(f.x, f.y);
+  }
+  // (Of the numbers: a NaN is left out.)
+  static __device__ __forceinline__ float top4(const uint4 (&q)[kVecs]) {
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(top2(q[0]), top2(q[1])), __hmax2(top2(q[2]), top2(q[3]))));
     return fmaxf(f.x, f.y);
   }
   static __device__ __forceinline__ Limit limit(float t) { return limit_of(__float2bfloat16_rn(t)); }
@@ -181,6 +194,7 @@ struct Scratch {
   int hist[256];
   int listed[3];         // of chunk c: entry c % 3, cleared while chunk c - 1 lists
   int count, picked, digit, need, bin;
+  uint32_t bound;
   float warp_m[kThreads / 32], warp_s[kThreads / 32];
   float m, s;            // this CTA's log-sum-exp parts
 };
@@ -296,6 +310,39 @@ __device__ __forceinline__ void sort_runs(int n, Scratch& sc) {
   }
 }
 
+// The r-th largest of the threads' keys: each warp's sorted, then the smallest key that
+// fewer than r keys exceed.  Ends with a barrier.
+__device__ __forceinline__ uint32_t rth_largest(uint32_t key, int r, Scratch& sc) {
+  const int lane = threadIdx.x & 31;
+  uint32_t* sorted = reinterpret_cast<uint32_t*>(sc.buf);
+  if (threadIdx.x == 0) sc.bound = 0xffffffffu;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+    for (int o = size / 2; o; o /= 2) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, key, o);
+      const bool keep_large = ((lane & o) == 0) == ((lane & size) == 0);
+      key = keep_large ? max(key, other) : min(key, other);
+    }
+  }
+  sorted[threadIdx.x] = key;
+  __syncthreads();
+  int above = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const uint32_t* run = sorted + 32 * w;
+    int here = 0;
+#pragma unroll
+    for (int o = 16; o; o /= 2) here += run[here + o - 1] > key ? o : 0;
+    above += here + (run[here] > key ? 1 : 0);
+  }
+  uint32_t low = above < r ? key : 0xffffffffu;
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (lane == 0) atomicMin(&sc.bound, low);
+  __syncthreads();
+  return sc.bound;
+}
+
 // emit(key, number of keys above it) for every key of the sorted runs.
 template <typename F>
 __device__ __forceinline__ void rank_runs(int n, const Scratch& sc, F emit) {
@@ -388,21 +435,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   };
   // The first threshold: the r-th largest of the threads' maxima over `cur`.
   auto threshold = [&](bool any, int r) {
-    float best = K::top(cur[0]);
-#pragma unroll
-    for (int j = 1; j < kVecs; ++j) best = fmaxf(best, K::top(cur[j]));
+    float best = K::top4(cur);
     if (!(best == best)) best = -INFINITY;
     // The maximum of rank r - 1 among all.  A NaN only lowers the maximum seen here,
     // which a bound may be; threads without an element come last.
-    sc.buf[tid] = (static_cast<u64>(any ? rising32(__float_as_uint(best)) : 0u) << 32) | static_cast<u64>(tid);
-    __syncwarp();
-    sort_runs(kThreads, sc);
-    __syncthreads();
-    rank_runs(kThreads, sc, [&](u64 key, int rank) {
-      if (rank == r - 1) sc.digit = static_cast<int>(key >> 32);
-    });
-    __syncthreads();
-    const uint32_t t = static_cast<uint32_t>(sc.digit);
+    const uint32_t t = rth_largest(any ? rising32(__float_as_uint(best)) : 0u, r, sc);
     limit_key = 0;
     limit = K::limit(__int_as_float(0x7fffffff));
     // As a value of the type, rounded down; candidates are at or above it.  (Below the
@@ -422,9 +459,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     if (full_key(key, i) > limit_key) sc.buf[atomicAdd(&sc.count, 1)] = full_key(key, i);
   };
   auto round_top = [&]() {
-    float tops = K::top(cur[0]);
-#pragma unroll
-    for (int j = 1; j < kVecs; ++j) tops = fmaxf(tops, K::top(cur[j]));
+    const float tops = K::top4(cur);
     if (tops > m) raise(tops);
   };
   auto add = [&](const uint4& q, u64 minus) {
@@ -654,7 +689,7 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   // keep half a chunk each.
   int parts = 1;
   const int sms = device_sm_count();
-  while (parts < kMaxParts && rows * parts * 2 <= 4 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
+  while (parts < kMaxParts && rows * parts * 2 <= 8 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);
