@@ -118,15 +118,35 @@ def load():
     return _lib
 
 
+def _raise(name, rc):
+    msg = load().sb_last_error().decode(errors="replace")
+    if rc == SB_EINVAL:
+        raise ValueError(f"{name}: {msg}")
+    raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
 def call(name, *args):
     """Invoke an entry point and turn a non-zero status into an exception."""
     rc = getattr(load(), name)(*args)
     if rc != SB_OK:
-        msg = load().sb_last_error().decode(errors="replace")
-        if rc == SB_EINVAL:
-            raise ValueError(f"{name}: {msg}")
-        raise RuntimeError(f"{name} failed ({rc}): {msg}")
+        _raise(name, rc)
     return rc
+
+
+def entry(name):
+    """``call`` of one entry point, looked up at its first use (for calls that are mostly
+    host time)."""
+    fn = None
+
+    def invoke(*args):
+        nonlocal fn
+        if fn is None:
+            fn = getattr(load(), name)
+        rc = fn(*args)
+        if rc != SB_OK:
+            _raise(name, rc)
+
+    return invoke
 
 
 def query(name, *args) -> int:
@@ -150,7 +170,7 @@ _HERE = contextlib.nullcontext()
 def on_device(device):
     """Context with `device` current; free when it already is."""
     import torch
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def dtype_code(dtype) -> int:

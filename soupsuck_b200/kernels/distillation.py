@@ -50,16 +50,16 @@ class _HeadDistillation(torch.autograd.Function):
         vocab, listed = weight.shape[0], indices.shape[1]
         padded = -(-width // 8) * 8
         dev = hidden.device
-        loss = torch.empty(rows, device=dev, dtype=SINGLE)
-        mass = torch.empty(rows, device=dev, dtype=SINGLE)
-        place = torch.empty(rows, device=dev, dtype=torch.int32)
-        du = torch.empty((rows, padded), device=dev, dtype=SINGLE) if gradient else None
+        loss = hidden.new_empty(rows, dtype=SINGLE)
+        mass = hidden.new_empty(rows, dtype=SINGLE)
+        place = hidden.new_empty(rows, dtype=torch.int32)
+        du = hidden.new_empty((rows, padded), dtype=SINGLE) if gradient else None
         if rows:
             x, w = _operand(hidden, padded), _operand(weight, padded)
             indices, logits = indices.contiguous(), logits.contiguous()
             lse = None if teacher_lse is None else teacher_lse.contiguous()
             nbytes = _lib.query("sb_distill_workspace_bytes", rows, padded, vocab, listed, int(gradient))
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            scratch = hidden.new_empty(nbytes, dtype=torch.uint8)
             _lib.call("sb_distill_forward", x.data_ptr(), rows, padded, w.data_ptr(), vocab,
                       _lib.wide_dtype_code(w.dtype), indices.data_ptr(), logits.data_ptr(),
                       _lib.wide_dtype_code(logits.dtype), listed, _lib.ptr(lse), temperature, loss.data_ptr(),
@@ -80,7 +80,7 @@ class _HeadDistillation(torch.autograd.Function):
         du, place = ctx.saved_tensors
         dtype, width = ctx.meta
         rows, padded = du.shape
-        dx = torch.empty((rows, padded), device=du.device, dtype=dtype)
+        dx = du.new_empty((rows, padded), dtype=dtype)
         if rows:
             with _lib.on_device(du.device):
                 g = grad_loss.contiguous()

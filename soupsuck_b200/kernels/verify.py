@@ -23,9 +23,8 @@ _NUMBERS = Operand(SINGLE, ndim=2, layout=None)
 _LENS = Operand(LONG, ndim=1, layout=None, optional=True)
 
 
-def _rows_unit(entry, name, t):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        refuse(entry, f"{name} has a strided last dimension; unit stride is required there")
+_CODES = {dtype: _lib.wide_dtype_code(dtype) for dtype in WIDE_FLOATS}
+_launch = _lib.entry("sb_verify_drafts")
 
 
 def verify_drafts(target_probs, draft_tokens, uniforms, noise, draft_probs=None, *, draft_lens=None):
@@ -36,38 +35,52 @@ def verify_drafts(target_probs, draft_tokens, uniforms, noise, draft_probs=None,
     S drafts.  tokens holds the accepted drafts, the token drawn behind them (-1 where the
     probabilities leave none) and -1 to its end.  A drafted token outside [0, V) is
     rejected."""
+    # (Host time counts here too: what is plainly right skips the rules.)
+    place = target_probs.get_device() if isinstance(target_probs, torch.Tensor) else -1
+    plain = (place >= 0 and target_probs.dim() == 3 and target_probs.dtype in _CODES
+             and _is(draft_tokens, LONG, 2, place) and _is(uniforms, SINGLE, 2, place) and _is(noise, SINGLE, 2, place)
+             and (draft_probs is None or _is(draft_probs, target_probs.dtype, 3, place))
+             and (draft_lens is None or _is(draft_lens, LONG, 1, place)))
+    if not plain:
+        _check(target_probs, draft_tokens, uniforms, noise, draft_probs, draft_lens)
+    batch, places, vocab = target_probs.shape
+    drafts = places - 1
+    if not (draft_tokens.shape == (batch, drafts) == uniforms.shape and noise.shape == (batch, vocab)
+            and (draft_probs is None or draft_probs.shape == (batch, drafts, vocab))
+            and (draft_lens is None or draft_lens.shape == (batch,))):
+        shape = lambda t: None if t is None else tuple(t.shape)  # noqa: E731
+        refuse("verify_drafts", f"target_probs {shape(target_probs)}, draft_tokens {shape(draft_tokens)}, uniforms "
+                                f"{shape(uniforms)}, noise {shape(noise)}, draft_probs {shape(draft_probs)} and draft_lens "
+                                f"{shape(draft_lens)} do not line up")
+    if vocab == 0:
+        refuse("verify_drafts", f"target_probs {tuple(target_probs.shape)} has an empty vocabulary")
+    t_batch, t_row, t_unit = target_probs.stride()
+    n_batch, n_unit = noise.stride()
+    d_batch, d_row, d_unit = (0, 0, 1) if draft_probs is None else draft_probs.stride()
+    if vocab > 1 and not t_unit == n_unit == d_unit == 1:
+        refuse("verify_drafts", "target_probs, noise or draft_probs has a strided last dimension; unit stride is "
+                                "required there")
+    device = target_probs.device
+    with _lib.on_device(device):
+        tokens_in, u = draft_tokens.contiguous(), uniforms.contiguous()
+        lens = None if draft_lens is None else draft_lens.contiguous()
+        accepted = tokens_in.new_empty(batch)
+        tokens = tokens_in.new_empty((batch, places))
+        if batch:
+            _launch(target_probs.data_ptr(), t_batch, t_row, _lib.ptr(draft_probs), d_batch, d_row,
+                    _CODES[target_probs.dtype], batch, drafts, vocab, tokens_in.data_ptr(), u.data_ptr(),
+                    noise.data_ptr(), n_batch, _lib.ptr(lens), accepted.data_ptr(), tokens.data_ptr(),
+                    _lib.raw_stream(device))
+    return accepted, tokens
+
+
+def _is(t, dtype, ndim, place):
+    return isinstance(t, torch.Tensor) and t.get_device() == place and t.dtype is dtype and t.dim() == ndim
+
+
+def _check(target_probs, draft_tokens, uniforms, noise, draft_probs, draft_lens):
     entry = "verify_drafts"
     device = target_probs.device if isinstance(target_probs, torch.Tensor) else None
     admit(entry, device, target_probs=(target_probs, _PROBS))
     admit(entry, device, draft_tokens=(draft_tokens, _TOKENS), uniforms=(uniforms, _NUMBERS), noise=(noise, _NUMBERS),
           draft_probs=(draft_probs, _LIKE[target_probs.dtype]), draft_lens=(draft_lens, _LENS))
-    batch, places, vocab = target_probs.shape
-    drafts = draft_tokens.shape[1]
-    lines_up = (places == drafts + 1 and draft_tokens.shape[0] == batch
-                and uniforms.shape == draft_tokens.shape and noise.shape == (batch, vocab)
-                and (draft_probs is None or draft_probs.shape == (batch, drafts, vocab))
-                and (draft_lens is None or draft_lens.shape == (batch,)))
-    if not lines_up:
-        refuse(entry, f"target_probs {tuple(target_probs.shape)}, draft_tokens {tuple(draft_tokens.shape)}, "
-                      f"uniforms {tuple(uniforms.shape)}, noise {tuple(noise.shape)}, draft_probs "
-                      f"{None if draft_probs is None else tuple(draft_probs.shape)} and draft_lens "
-                      f"{None if draft_lens is None else tuple(draft_lens.shape)} do not line up")
-    if vocab == 0:
-        refuse(entry, f"target_probs {tuple(target_probs.shape)} has an empty vocabulary")
-    _rows_unit(entry, "target_probs", target_probs)
-    _rows_unit(entry, "noise", noise)
-    if draft_probs is not None:
-        _rows_unit(entry, "draft_probs", draft_probs)
-    with _lib.on_device(device):
-        tokens_in, u = draft_tokens.contiguous(), uniforms.contiguous()
-        lens = None if draft_lens is None else draft_lens.contiguous()
-        accepted = torch.empty(batch, device=device, dtype=LONG)
-        tokens = torch.empty((batch, drafts + 1), device=device, dtype=LONG)
-        if batch:
-            q = draft_probs
-            _lib.call("sb_verify_drafts", target_probs.data_ptr(), target_probs.stride(0), target_probs.stride(1),
-                      _lib.ptr(q), 0 if q is None else q.stride(0), 0 if q is None else q.stride(1),
-                      _lib.wide_dtype_code(target_probs.dtype), batch, drafts, vocab, tokens_in.data_ptr(),
-                      u.data_ptr(), noise.data_ptr(), noise.stride(0), _lib.ptr(lens), accepted.data_ptr(),
-                      tokens.data_ptr(), _lib.raw_stream(device))
-    return accepted, tokens
