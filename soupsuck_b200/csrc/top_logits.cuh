@@ -15,7 +15,9 @@
 // the row, so the first round is an even sample of it; with s of n elements sampled, the
 // r-th largest of the threads' maxima, r = k s / n + 2.5 sqrt(k s / n) + 3, leaves a few
 // times k candidates and almost never fewer than k.  Where it does leave fewer, or the
-// list overflows (a row of equal or masked logits), the row is read again with the
+// list overflows (a row of equal or masked logits; where a cluster shares a row, where
+// fewer than k of all parts' candidates lie above each part's threshold), the row is read
+// again with the
 // threshold that cannot fail: the k-th largest of the threads' maxima over a first chunk
 // in index order, raised to the k-th of all so far whenever the candidates have doubled;
 // the list then holds a whole chunk and is worked off at its end, so any row is handled.
@@ -195,6 +197,7 @@ struct Scratch {
   int listed[3];         // of chunk c: entry c % 3, cleared while chunk c - 1 lists
   int count, picked, digit, need, bin;
   uint32_t bound;
+  u64 limit;             // keys at or below it may be missing among the candidates
   float warp_m[kThreads / 32], warp_s[kThreads / 32];
   float m, s;            // this CTA's log-sum-exp parts
 };
@@ -361,16 +364,18 @@ __device__ __forceinline__ void rank_runs(int n, const Scratch& sc, F emit) {
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
+// CLUSTER: a cluster of CTAs shares each row (else one CTA per row, whose code then keeps
+// nothing for a second attempt and needs fewer registers).
+template <typename T, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
                                                           int k, float scale, float inv_tau, void* __restrict__ values,
                                                           int64_t* __restrict__ indices, float* __restrict__ lse) {
   using K = Kind<T>;
   constexpr int kBits = 8 * sizeof(T);
   __shared__ __align__(16) Scratch sc;
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = static_cast<int>(cluster.num_blocks());
-  const int part = static_cast<int>(cluster.block_rank());
+  const int parts = CLUSTER ? static_cast<int>(cluster.num_blocks()) : 1;
+  const int part = CLUSTER ? static_cast<int>(cluster.block_rank()) : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t low16 = sizeof(T) == 4 ? 0xff800000u : (K::kBrain ? 0xff80ff80u : 0xfc00fc00u);
   const uint4 nothing = make_uint4(low16, low16, low16, low16);  // -inf
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   bool safe = true;
   {
     // The guess (its first round is loaded already).
-    const float share = rounds > 1 ? static_cast<float>(k) / rounds : static_cast<float>(k);
+    const float share = static_cast<float>(k) / max(rounds * parts, 1);
     const int r = min(k, static_cast<int>(share + 2.5f * sqrtf(share)) + 3);
     threshold(left > 0, r);
     if (ends && tid < head) one(tid);
@@ -537,11 +542,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     const int listed = sc.listed[0];
     if (listed <= kChunk) {
       const int count = work_off(listed * K::kPer);
-      // (The tail's elements are still to come, the guess counts without them.)
-      safe = count < k && limit_key != 0;
+      // (The tail's elements are still to come, the guess counts without them.  A part
+      // among others need not have k: the parts are judged together below.)
+      safe = parts == 1 && count < k && limit_key != 0;
     }
   }
-  if (safe) {
+  int kept = 0, rank = 0;
+  u64 own_key = 0;
+  for (bool again = false;; again = true) {
+  if (safe || (CLUSTER && again)) {
     const uint4* xv = reinterpret_cast<const uint4*>(x + head) + w0 + tid;
     const int own = w1 - w0 - tid;  // vectors from this thread's first on
     __syncthreads();
@@ -613,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   if (n > kRankable) n = cut(n);
   sort_runs(n, sc);
   __syncthreads();
-  const int kept = n < k ? n : k;
+  kept = n < k ? n : k;
   rank_runs(n, sc, [&](u64 key, int rank) {
     if (rank < kept) sc.sel[rank] = key;
   });
@@ -625,8 +634,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
     for (int w = 0; w < kThreads / 32; ++w) sum += sc.warp_s[w] * exp2_fast(sc.warp_m[w] - big);
     sc.m = big;
     sc.s = sum;
+    sc.limit = kept == k || safe || again ? 0 : limit_key;
   }
-  if (parts > 1) {
+  if constexpr (CLUSTER) {
     cluster.sync();
   } else {
     __syncthreads();
@@ -634,31 +644,46 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
   // An entry's place in the output: its place here and the entries above it in the
   // other parts' lists, searched side by side (a remote load takes about as long as
   // eight at once).
-  for (int i = tid; i < kept; i += kThreads) {
-    const u64 key = sc.sel[i];
-    int rank = i;
-    if (parts > 1) {
-      int above[kMaxParts] = {};
-      for (int o = 1 << (31 - __clz(k)); o; o >>= 1) {
-        u64 at[kMaxParts];
+  static_assert(kMaxK <= kThreads, "an entry per thread");
+  rank = tid;
+  own_key = tid < kept ? sc.sel[tid] : 0;
+  if constexpr (!CLUSTER) {
+    break;
+  } else {
+  auto above_in = [&](u64 key) {
+    int above[kMaxParts] = {};
+    for (int o = 1 << (31 - __clz(k)); o; o >>= 1) {
+      u64 at[kMaxParts];
 #pragma unroll
-        for (int c = 0; c < kMaxParts; ++c) {
-          if (c < parts && above[c] + o <= k) at[c] = cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1];
-        }
-#pragma unroll
-        for (int c = 0; c < kMaxParts; ++c) above[c] += c < parts && above[c] + o <= k && at[c] > key ? o : 0;
+      for (int c = 0; c < kMaxParts; ++c) {
+        if (c < parts && above[c] + o <= k) at[c] = cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1];
       }
-      rank = 0;
 #pragma unroll
-      for (int c = 0; c < kMaxParts; ++c) rank += above[c];
+      for (int c = 0; c < kMaxParts; ++c) above[c] += c < parts && above[c] + o <= k && at[c] > key ? o : 0;
     }
-    if (rank < k) {
-      K::store(values, row * k + rank, static_cast<uint32_t>(key >> 32));
-      indices[row * k + rank] = static_cast<int64_t>(0xffffffffull - (key & 0xffffffffull));
-    }
+    int sum = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxParts; ++c) sum += above[c];
+    return sum;
+  };
+  if (tid < kept) rank = above_in(own_key);
+  // Nothing is missing if k entries lie above every part's limit.
+  u64 limit_of_all = lane < parts ? cluster.map_shared_rank(&sc, lane)->limit : 0;
+  for (int o = kMaxParts / 2; o; o >>= 1) {
+    const u64 other = __shfl_xor_sync(0xffffffffu, limit_of_all, o);
+    limit_of_all = other > limit_of_all ? other : limit_of_all;
+  }
+  limit_of_all = __shfl_sync(0xffffffffu, limit_of_all, 0);
+  if (limit_of_all == 0 || above_in(limit_of_all) >= k) break;
+  cluster.sync();  // all have read the lists that are made anew
+  }
+  }
+  if (tid < kept && rank < k) {
+    K::store(values, row * k + rank, static_cast<uint32_t>(own_key >> 32));
+    indices[row * k + rank] = static_cast<int64_t>(0xffffffffull - (own_key & 0xffffffffull));
   }
   if (part == 0 && warp == 0) {
-    const Scratch* from = lane < parts ? cluster.map_shared_rank(&sc, lane) : &sc;
+    const Scratch* from = CLUSTER && lane < parts ? cluster.map_shared_rank(&sc, lane) : &sc;
     u64 top = from->sel[0];
     float big = from->m, sum = lane < parts ? from->s : 0.0f;
     for (int o = kMaxParts / 2; o; o >>= 1) {
@@ -679,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) top_kernel(const T* __restri
                                                   : topv * inv_tau;
     }
   }
-  if (parts > 1) cluster.sync();  // the others' lists stay until all have read them
+  if (CLUSTER) cluster.sync();  // the others' lists stay until all have read them
 }
 
 template <typename T>
@@ -699,8 +724,8 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   attr[0].val.clusterDim.x = parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, top_kernel<T>, static_cast<const T*>(logits), v, pitch, k,
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, parts > 1 ? top_kernel<T, true> : top_kernel<T, false>, static_cast<const T*>(logits), v, pitch, k,
                                            1.4426950408889634f / temperature, 1.0f / temperature, values, indices, lse);
   if (e != cudaSuccess) return fail(SB_ECUDA, std::string("top_kernel: ") + cudaGetErrorString(e));
   count_launch();
