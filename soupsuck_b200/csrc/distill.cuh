@@ -433,9 +433,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(
   const int* row_columns = columns + (row_base + at) * k;
   for (int j = lane; j < m; j += 32) {
     const float x = z[j] / f;
-    z[j] = x;  // (read back below by the same lane)
+    z[j] = x;
     if (even) dz[at * pitch + row_columns[j]] = static_cast<uint16_t>(dense::pack2<BF16>(x, 0.0f) & 0xffffu);
   }
+  __syncwarp();
   // What the rounding to 16 bits takes from the listed columns is most of dz's error; the
   // largest four amounts are kept, for the product's sums.
   uint64_t before = ~0ull;
