@@ -12,9 +12,9 @@
 //   * selection: vectors with an element at or above a threshold go to a list in shared
 //     memory, which is sorted out when the row has been read.
 // The threshold is a guess.  The 32 streams of a CTA (warp, vector) lie side by side in
-// the row, so the first round is an even sample of it; with s of n elements sampled, the
-// r-th largest of the threads' maxima, r = k s / n + 2.5 sqrt(k s / n) + 3, leaves a few
-// times k candidates and almost never fewer than k.  Where it does leave fewer, or the
+// the row, so the first round is an even sample of it; with s of n elements sampled, a
+// threshold that k s / n + 2.5 sqrt(k s / n) + 3 of them pass (taken from the threads'
+// maxima) leaves a few times k candidates and almost never fewer than k.  Where it does leave fewer, or the
 // list overflows (a row of equal or masked logits; where a cluster shares a row, where
 // fewer than k of all parts' candidates lie above each part's threshold), the row is read
 // again with the
@@ -364,17 +364,18 @@ __device__ __forceinline__ void rank_runs(int n, const Scratch& sc, F emit) {
   }
 }
 
-// CLUSTER: a cluster of CTAs shares each row (else one CTA per row, whose code then keeps
+// PARTS: the CTAs of a cluster that share each row (with one per row, the code keeps
 // nothing for a second attempt and needs fewer registers).
-template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
                                                           int k, float scale, float inv_tau, void* __restrict__ values,
                                                           int64_t* __restrict__ indices, float* __restrict__ lse) {
   using K = Kind<T>;
   constexpr int kBits = 8 * sizeof(T);
   __shared__ __align__(16) Scratch sc;
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = CLUSTER ? static_cast<int>(cluster.num_blocks()) : 1;
+  constexpr bool CLUSTER = PARTS > 1;
+  constexpr int parts = PARTS;
   const int part = CLUSTER ? static_cast<int>(cluster.block_rank()) : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t low16 = sizeof(T) == 4 ? 0xff800000u : (K::kBrain ? 0xff80ff80u : 0xfc00fc00u);
@@ -498,8 +499,12 @@ __global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(con
   bool safe = true;
   {
     // The guess (its first round is loaded already).
+    // `want` elements of the sample above the threshold; as they fall into the threads at
+    // random, so many threads' maxima are above it too.  (k maxima would never fail.)
     const float share = static_cast<float>(k) / max(rounds * parts, 1);
-    const int r = min(k, static_cast<int>(share + 2.5f * sqrtf(share)) + 3);
+    const float want = share + 2.5f * sqrtf(share) + 3.0f;
+    const float groups = static_cast<float>(max(min(kThreads, w1 - w0), 1));
+    const int r = min(k, static_cast<int>(groups * (1.0f - __expf(-want / groups))) + 1);
     threshold(left > 0, r);
     if (ends && tid < head) one(tid);
     // Every stream of the thread full (all but the part's last ones): no bounds to look at.
@@ -650,31 +655,34 @@ __global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(con
   if constexpr (!CLUSTER) {
     break;
   } else {
-  auto above_in = [&](u64 key) {
-    int above[kMaxParts] = {};
-    for (int o = 1 << (31 - __clz(k)); o; o >>= 1) {
-      u64 at[kMaxParts];
+  const int first_o = 1 << (31 - __clz(k));
+  if (tid < kept) {
+    int above[parts] = {};
+    for (int o = first_o; o; o >>= 1) {
+      u64 at[parts];
 #pragma unroll
-      for (int c = 0; c < kMaxParts; ++c) {
-        if (c < parts && above[c] + o <= k) at[c] = cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1];
-      }
+      for (int c = 0; c < parts; ++c) at[c] = above[c] + o <= k ? cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1] : 0;
 #pragma unroll
-      for (int c = 0; c < kMaxParts; ++c) above[c] += c < parts && above[c] + o <= k && at[c] > key ? o : 0;
+      for (int c = 0; c < parts; ++c) above[c] += at[c] > own_key ? o : 0;
     }
-    int sum = 0;
+    rank = 0;
 #pragma unroll
-    for (int c = 0; c < kMaxParts; ++c) sum += above[c];
-    return sum;
-  };
-  if (tid < kept) rank = above_in(own_key);
-  // Nothing is missing if k entries lie above every part's limit.
-  u64 limit_of_all = lane < parts ? cluster.map_shared_rank(&sc, lane)->limit : 0;
-  for (int o = kMaxParts / 2; o; o >>= 1) {
+    for (int c = 0; c < parts; ++c) rank += above[c];
+  }
+  // Nothing is missing if k entries lie above every part's limit (lane c counts part c's).
+  const Scratch* theirs = cluster.map_shared_rank(&sc, lane & (parts - 1));
+  u64 limit_of_all = theirs->limit;
+#pragma unroll
+  for (int o = parts / 2; o; o >>= 1) {
     const u64 other = __shfl_xor_sync(0xffffffffu, limit_of_all, o);
     limit_of_all = other > limit_of_all ? other : limit_of_all;
   }
-  limit_of_all = __shfl_sync(0xffffffffu, limit_of_all, 0);
-  if (limit_of_all == 0 || above_in(limit_of_all) >= k) break;
+  if (limit_of_all == 0) break;
+  int above = 0;
+  for (int o = first_o; o; o >>= 1) above += above + o <= k && theirs->sel[above + o - 1] > limit_of_all ? o : 0;
+#pragma unroll
+  for (int o = parts / 2; o; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+  if (above >= k) break;
   cluster.sync();  // all have read the lists that are made anew
   }
   }
@@ -686,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(con
     const Scratch* from = CLUSTER && lane < parts ? cluster.map_shared_rank(&sc, lane) : &sc;
     u64 top = from->sel[0];
     float big = from->m, sum = lane < parts ? from->s : 0.0f;
-    for (int o = kMaxParts / 2; o; o >>= 1) {
+    for (int o = parts / 2; o; o >>= 1) {
       const u64 t = __shfl_xor_sync(0xffffffffu, top, o);
       top = t > top ? t : top;
       const float om = __shfl_xor_sync(0xffffffffu, big, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
@@ -710,11 +718,15 @@ __global__ void __launch_bounds__(kThreads, CLUSTER ? 3 : kPerSm) top_kernel(con
 template <typename T>
 int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, float temperature, void* values,
            int64_t* indices, float* lse, cudaStream_t st) {
-  // Few rows are split over a cluster (at most the portable eight CTAs) while the parts
-  // keep half a chunk each.
+  // Few rows are split over a cluster (at most the portable eight CTAs): to an SM's one
+  // CTA in parts of half a chunk, to eight in parts of two (300 rows of 151936 fp16: four
+  // parts 40 us, two 51; 600 rows in two 83, in one 68).
   int parts = 1;
-  const int sms = device_sm_count();
-  while (parts < kMaxParts && rows * parts * 2 <= 8 * sms && v / (parts * 2) >= kChunk * Kind<T>::kPer / 2) parts *= 2;
+  const int64_t sms = device_sm_count(), chunk = kChunk * Kind<T>::kPer;
+  while (parts < kMaxParts && rows * parts * 2 <= 8 * sms &&
+         v / (parts * 2) >= (rows * parts * 2 <= sms ? chunk / 2 : 2 * chunk)) {
+    parts *= 2;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);
@@ -725,7 +737,8 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, parts > 1 ? top_kernel<T, true> : top_kernel<T, false>, static_cast<const T*>(logits), v, pitch, k,
+  auto kern = parts == 1 ? top_kernel<T, 1> : parts == 2 ? top_kernel<T, 2> : parts == 4 ? top_kernel<T, 4> : top_kernel<T, 8>;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(logits), v, pitch, k,
                                            1.4426950408889634f / temperature, 1.0f / temperature, values, indices, lse);
   if (e != cudaSuccess) return fail(SB_ECUDA, std::string("top_kernel: ") + cudaGetErrorString(e));
   count_launch();
