@@ -464,10 +464,6 @@ __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(c
     s += exp2_fast(fmaf(f, scale, -m2));
     if (full_key(key, i) > limit_key) sc.buf[atomicAdd(&sc.count, 1)] = full_key(key, i);
   };
-  auto round_top = [&]() {
-    const float tops = K::top4(cur);
-    if (tops > m) raise(tops);
-  };
   auto add = [&](const uint4& q, u64 minus) {
 #pragma unroll
     for (int i = 0; i < K::kPer; i += 2) {
@@ -510,32 +506,45 @@ __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(c
     // Every stream of the thread full (all but the part's last ones): no bounds to look at.
     auto stream = [&](auto whole) {
       constexpr bool full = decltype(whole)::value;
-      const uint4* at = xs;
-      int64_t index = head + (w0 + (warp * rounds) * 32 + lane) * static_cast<int64_t>(K::kPer);
-      for (int c = 0; c < rounds; ++c) {
-        round_top();
-        const u64 minus = pack2(-m2, -m2);
+      const uint4* at = xs;  // of the round that is loaded next
+      const int stride = kWarps * rounds * 32;
+      auto load = [&](uint4 (&q)[kVecs], int c) {
         at += 32;
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
-          const uint4 q = cur[j];
           if (full) {
-            if (c + 1 < rounds) cur[j] = __ldcs(at + j * kWarps * rounds * 32);
+            if (c < rounds) q[j] = __ldcs(at + j * stride);
           } else {
-            const int w = (j * kWarps * rounds + c + 1) * 32;
-            cur[j] = c + 1 < rounds && w < left ? __ldcs(xs + w) : nothing;
+            q[j] = c < rounds && j * stride + c * 32 < left ? __ldcs(at + j * stride) : nothing;
           }
-          if (K::above(q, limit) && (full || (j * kWarps * rounds + c) * 32 < left)) {
+        }
+      };
+      auto eat = [&](const uint4 (&q)[kVecs], int c) {
+        const float tops = K::top4(q);
+        if (tops > m) raise(tops);
+        const u64 minus = pack2(-m2, -m2);
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+          if (K::above(q[j], limit) && (full || j * stride + c * 32 < left)) {
             const int slot = atomicAdd(&sc.listed[0], 1);
             if (slot < kChunk) {
-              sc.list[slot] = q;
-              sc.list_at[slot] = static_cast<int>(index) + (j * kWarps * rounds + c) * 32 * K::kPer;
-            } else {
-              c = rounds;  // overflow: the other form will do it
+              sc.list[slot] = q[j];
+              sc.list_at[slot] = head + (w0 + warp * rounds * 32 + lane + j * stride + c * 32) * K::kPer;
             }
           }
-          add(q, minus);
+          add(q[j], minus);
         }
+      };
+      // Two rounds in registers by turns.  (Past an overflow of the list it is of no use to
+      // go on: the other form will do it.)
+      uint4 other[kVecs];
+      for (int c = 0; c < rounds; c += 2) {
+        load(other, c + 1);
+        eat(cur, c);
+        if (c + 1 >= rounds) break;
+        load(cur, c + 2);
+        eat(other, c + 1);
+        if (*reinterpret_cast<volatile int*>(&sc.listed[0]) > kChunk) break;
       }
     };
     if (__all_sync(0xffffffffu, ((kVecs - 1) * kWarps * rounds + rounds - 1) * 32 < left)) {
@@ -580,7 +589,8 @@ __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(c
     for (int first = 0; first < w1 - w0; first += kChunk) {
       const int next_turn = turn == 2 ? 0 : turn + 1;
       if (tid == 0) sc.listed[next_turn] = 0;  // read last before the previous barrier
-      round_top();
+      const float tops = K::top4(cur);
+      if (tops > m) raise(tops);
       const u64 minus = pack2(-m2, -m2);
 #pragma unroll
       for (int j = 0; j < kVecs; ++j) {
