@@ -211,6 +211,35 @@ def test_evaluation_matches_training_and_repeats():
     assert torch.equal(a, first[2]) and torch.allclose(b.float(), 2 * a.float(), rtol=2 ** -10, atol=2 ** -23)
 
 
+def test_more_rows_than_one_block_holds():
+    """15000 rows of 151936 tokens are worked off in two blocks (4 GB of exponentials hold 14080).  Rows
+    do not depend on one another: losses equal those of two smaller calls exactly; the product's splits
+    differ with the rows, so gradients may differ by their runs: 64 tensor-core additions each, one ulp
+    of a magnitude sum of at most 2 max|W| apiece on either side, and one rounding to fp16."""
+    from soupsuck_b200.kernels import fused_linear_distillation
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows, hidden, vocab, k = 15000, 64, 151936, 4
+    x = torch.randn((rows, hidden), device="cuda", generator=g).half()
+    w = (torch.randn((vocab, hidden), device="cuda", generator=g) / 8).half()
+    indices = torch.randint(vocab // 4, (rows, k), device="cuda", generator=g) + torch.arange(k, device="cuda") * (vocab // 4)
+    logits = torch.rand((rows, k), device="cuda", generator=g) * 3
+    lse = torch.logsumexp(logits, 1) + 0.3
+    indices[::7] = -1
+
+    def call(part):
+        leaf = x[part].clone().requires_grad_()
+        loss, mass = fused_linear_distillation(leaf, w, indices[part], logits[part], lse[part], validate=False)
+        return loss.detach(), mass, torch.autograd.grad(loss.sum(), leaf)[0]
+
+    whole, first, second = call(slice(None)), call(slice(0, 8000)), call(slice(8000, None))
+    for got, a, b in zip(whole[:2], first, second):
+        assert torch.equal(got, torch.cat([a, b]))
+    dx, parts = whole[2].float(), torch.cat([first[2], second[2]]).float()
+    assert torch.isfinite(dx).all() and not dx[::7].any()
+    runs = 2 * 64 * 2.0 ** -23 * 2 * w.float().abs().max()
+    assert ((dx - parts).abs() <= 2.0 ** -10 * parts.abs() + runs).all()
+
+
 def test_rows_with_nan_stay_apart():
     from soupsuck_b200.kernels import fused_linear_distillation
     x, w, indices, logits, lse, upstream = _inputs(20, 64, 700, 6)
