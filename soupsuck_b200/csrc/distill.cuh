@@ -26,6 +26,10 @@
 // use that exponent.  Keeping the exponentials instead of forming the logits a second
 // time saves a third of the matrix work.
 // Backward.  dhidden = upstream * du, rounded once.
+//
+// Measured (one pass, V = 151936): 1221 answered of 3300 rows, H = 1536: logits 432, product
+// 417, all others 62 us; 48 rows 95, 87 and 45; the two products are what bounds it
+// (dense_pair.cuh), the small kernels (4 to 20 us each) wait for dependent loads.
 #pragma once
 
 #include <type_traits>

@@ -21,8 +21,12 @@
 // threshold that cannot fail: the k-th largest of the threads' maxima over a first chunk
 // in index order, raised to the k-th of all so far whenever the candidates have doubled;
 // the list then holds a whole chunk and is worked off at its end, so any row is handled.
-// 3300 rows of 151936 fp16, k = 64: reading takes 154 us, the safe form alone 259 us
-// (taking the vectors apart in the loop instead of listing them 703 us).
+//
+// Measured, k = 64 (copy rate in brackets): 3300 rows of 151936 fp16 200 us (154; the safe
+// form alone 259, taking the vectors apart in the loop instead of listing them 703), fp32
+// about 330 (307), one row 10.  What bounds it: for 16-bit logits instruction issue and the
+// exponentials' unit, each about two thirds busy; for fp32 memory; for one row the chain of
+// load, threshold, sort and exchange.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -66,7 +70,9 @@ template <typename T> struct Kind;
 template <> struct Kind<float> {
   static constexpr int kPer = 4;
   static constexpr bool kBrain = false;
-  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising32(reinterpret_cast<const uint32_t*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) {
+    return rising32(reinterpret_cast<const uint32_t*>(v)[i]);
+  }
   static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising32(__float_as_uint(f)); }
   struct Limit { float t; };
   static __device__ __forceinline__ float value(const uint4& v, int i) {
@@ -108,7 +114,9 @@ template <typename T, typename T2> struct Kind16 {
 
 template <> struct Kind<__half> : Kind16<__half, __half2> {
   static constexpr bool kBrain = false;
-  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising(reinterpret_cast<const unsigned short*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) {
+    return rising(reinterpret_cast<const unsigned short*>(v)[i]);
+  }
   static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising(__half_as_ushort(__float2half_rd(f))); }
   static __device__ __forceinline__ uint32_t rising(uint32_t b) {
     if ((b & 0x7fffu) == 0u) return 0x80000000u;
@@ -140,7 +148,9 @@ template <> struct Kind<__half> : Kind16<__half, __half2> {
 
 template <> struct Kind<__nv_bfloat16> : Kind16<__nv_bfloat16, __nv_bfloat162> {
   static constexpr bool kBrain = true;
-  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) { return rising(reinterpret_cast<const unsigned short*>(v)[i]); }
+  static __device__ __forceinline__ uint32_t stored_key(const uint4* v, int i) {
+    return rising(reinterpret_cast<const unsigned short*>(v)[i]);
+  }
   static __device__ __forceinline__ uint32_t key_at_most(float f) { return rising(__bfloat16_as_ushort(__float2bfloat16_rd(f))); }
   static __device__ __forceinline__ uint32_t rising(uint32_t b) {
     if ((b & 0x7fffu) == 0u) return 0x80000000u;
@@ -564,137 +574,137 @@ __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(c
   int kept = 0, rank = 0;
   u64 own_key = 0;
   for (bool again = false;; again = true) {
-  if (safe || (CLUSTER && again)) {
-    const uint4* xv = reinterpret_cast<const uint4*>(x + head) + w0 + tid;
-    const int own = w1 - w0 - tid;  // vectors from this thread's first on
-    __syncthreads();
-    if (tid == 0) sc.count = sc.listed[0] = sc.listed[1] = sc.listed[2] = 0;
-    m = -1e30f;
-    m2 = fmaxf(-1e30f * scale, -3e38f);
-    s = 0.0f;
-    s2 = 0;
-    auto load = [&](int first) {
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j) {
-        const int w = first + j * kThreads;
-        cur[j] = w < own ? __ldg(xv + w) : nothing;
-      }
-    };
-    load(0);
-    threshold(own > 0, k);
-    // The head before the vectors and the tail behind them: in index order, as the
-    // strict threshold asks.
-    if (ends && tid < head) one(tid);
-    int turn = 0;
-    for (int first = 0; first < w1 - w0; first += kChunk) {
-      const int next_turn = turn == 2 ? 0 : turn + 1;
-      if (tid == 0) sc.listed[next_turn] = 0;  // read last before the previous barrier
-      const float tops = K::top4(cur);
-      if (tops > m) raise(tops);
-      const u64 minus = pack2(-m2, -m2);
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j) {
-        if (K::above(cur[j], limit) && first + j * kThreads < own) {
-          const int at = atomicAdd(&sc.listed[turn], 1);
-          sc.list[at] = cur[j];
-          sc.list_at[at] = head + (w0 + tid + first + j * kThreads) * K::kPer;
-        }
-        add(cur[j], minus);
-      }
-      load(first + kChunk);
+    if (safe || (CLUSTER && again)) {
+      const uint4* xv = reinterpret_cast<const uint4*>(x + head) + w0 + tid;
+      const int own = w1 - w0 - tid;  // vectors from this thread's first on
       __syncthreads();
-      const int listed = sc.listed[turn] * K::kPer;
-      turn = next_turn;
-      if (listed) {
-        const int count = work_off(listed);
-        if (count >= 2 * k) cut(count);
-        // Strictly: later vectors have higher indices.
-        if (limit_key & 0xffffffffull) set_limit(static_cast<uint32_t>(limit_key >> 32));
+      if (tid == 0) sc.count = sc.listed[0] = sc.listed[1] = sc.listed[2] = 0;
+      m = -1e30f;
+      m2 = fmaxf(-1e30f * scale, -3e38f);
+      s = 0.0f;
+      s2 = 0;
+      auto load = [&](int first) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+          const int w = first + j * kThreads;
+          cur[j] = w < own ? __ldg(xv + w) : nothing;
+        }
+      };
+      load(0);
+      threshold(own > 0, k);
+      // The head before the vectors and the tail behind them: in index order, as the
+      // strict threshold asks.
+      if (ends && tid < head) one(tid);
+      int turn = 0;
+      for (int first = 0; first < w1 - w0; first += kChunk) {
+        const int next_turn = turn == 2 ? 0 : turn + 1;
+        if (tid == 0) sc.listed[next_turn] = 0;  // read last before the previous barrier
+        const float tops = K::top4(cur);
+        if (tops > m) raise(tops);
+        const u64 minus = pack2(-m2, -m2);
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+          if (K::above(cur[j], limit) && first + j * kThreads < own) {
+            const int at = atomicAdd(&sc.listed[turn], 1);
+            sc.list[at] = cur[j];
+            sc.list_at[at] = head + (w0 + tid + first + j * kThreads) * K::kPer;
+          }
+          add(cur[j], minus);
+        }
+        load(first + kChunk);
+        __syncthreads();
+        const int listed = sc.listed[turn] * K::kPer;
+        turn = next_turn;
+        if (listed) {
+          const int count = work_off(listed);
+          if (count >= 2 * k) cut(count);
+          // Strictly: later vectors have higher indices.
+          if (limit_key & 0xffffffffull) set_limit(static_cast<uint32_t>(limit_key >> 32));
+        }
       }
     }
-  }
-  if (ends && tid < v - tail) one(tail + tid);
+    if (ends && tid < v - tail) one(tail + tid);
 
-  // Log-sum-exp of this CTA.
-  {
-    const float2 both = unpack2(s2);
-    s += both.x + both.y;
-  }
-  for (int o = 16; o; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m2, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-    const float big = fmaxf(m2, om);
-    s = s * exp2_fast(m2 - big) + os * exp2_fast(om - big);
-    m2 = big;
-  }
-  if (lane == 0) {
-    sc.warp_m[warp] = m2;
-    sc.warp_s[warp] = s;
-  }
-  __syncthreads();
-  // This CTA's k largest in falling order.
-  int n = sc.count;
-  __syncthreads();
-  if (n > kRankable) n = cut(n);
-  sort_runs(n, sc);
-  __syncthreads();
-  kept = n < k ? n : k;
-  rank_runs(n, sc, [&](u64 key, int rank) {
-    if (rank < kept) sc.sel[rank] = key;
-  });
-  for (int i = kept + tid; i < kMaxK; i += kThreads) sc.sel[i] = 0;
-  if (tid == 0) {
-    float big = sc.warp_m[0];
-    for (int w = 1; w < kThreads / 32; ++w) big = fmaxf(big, sc.warp_m[w]);
-    float sum = 0.0f;
-    for (int w = 0; w < kThreads / 32; ++w) sum += sc.warp_s[w] * exp2_fast(sc.warp_m[w] - big);
-    sc.m = big;
-    sc.s = sum;
-    sc.limit = kept == k || safe || again ? 0 : limit_key;
-  }
-  if constexpr (CLUSTER) {
-    cluster.sync();
-  } else {
-    __syncthreads();
-  }
-  // An entry's place in the output: its place here and the entries above it in the
-  // other parts' lists, searched side by side (a remote load takes about as long as
-  // eight at once).
-  static_assert(kMaxK <= kThreads, "an entry per thread");
-  rank = tid;
-  own_key = tid < kept ? sc.sel[tid] : 0;
-  if constexpr (!CLUSTER) {
-    break;
-  } else {
-  const int first_o = 1 << (31 - __clz(k));
-  if (tid < kept) {
-    int above[parts] = {};
-    for (int o = first_o; o; o >>= 1) {
-      u64 at[parts];
-#pragma unroll
-      for (int c = 0; c < parts; ++c) at[c] = above[c] + o <= k ? cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1] : 0;
-#pragma unroll
-      for (int c = 0; c < parts; ++c) above[c] += at[c] > own_key ? o : 0;
+    // Log-sum-exp of this CTA.
+    {
+      const float2 both = unpack2(s2);
+      s += both.x + both.y;
     }
-    rank = 0;
+    for (int o = 16; o; o >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m2, o), os = __shfl_xor_sync(0xffffffffu, s, o);
+      const float big = fmaxf(m2, om);
+      s = s * exp2_fast(m2 - big) + os * exp2_fast(om - big);
+      m2 = big;
+    }
+    if (lane == 0) {
+      sc.warp_m[warp] = m2;
+      sc.warp_s[warp] = s;
+    }
+    __syncthreads();
+    // This CTA's k largest in falling order.
+    int n = sc.count;
+    __syncthreads();
+    if (n > kRankable) n = cut(n);
+    sort_runs(n, sc);
+    __syncthreads();
+    kept = n < k ? n : k;
+    rank_runs(n, sc, [&](u64 key, int rank) {
+      if (rank < kept) sc.sel[rank] = key;
+    });
+    for (int i = kept + tid; i < kMaxK; i += kThreads) sc.sel[i] = 0;
+    if (tid == 0) {
+      float big = sc.warp_m[0];
+      for (int w = 1; w < kThreads / 32; ++w) big = fmaxf(big, sc.warp_m[w]);
+      float sum = 0.0f;
+      for (int w = 0; w < kThreads / 32; ++w) sum += sc.warp_s[w] * exp2_fast(sc.warp_m[w] - big);
+      sc.m = big;
+      sc.s = sum;
+      sc.limit = kept == k || safe || again ? 0 : limit_key;
+    }
+    if constexpr (CLUSTER) {
+      cluster.sync();
+    } else {
+      __syncthreads();
+    }
+    // An entry's place in the output: its place here and the entries above it in the
+    // other parts' lists, searched side by side (a remote load takes about as long as
+    // eight at once).
+    static_assert(kMaxK <= kThreads, "an entry per thread");
+    rank = tid;
+    own_key = tid < kept ? sc.sel[tid] : 0;
+    if constexpr (!CLUSTER) {
+      break;
+    } else {
+      const int first_o = 1 << (31 - __clz(k));
+      if (tid < kept) {
+        int above[parts] = {};
+        for (int o = first_o; o; o >>= 1) {
+          u64 at[parts];
 #pragma unroll
-    for (int c = 0; c < parts; ++c) rank += above[c];
-  }
-  // Nothing is missing if k entries lie above every part's limit (lane c counts part c's).
-  const Scratch* theirs = cluster.map_shared_rank(&sc, lane & (parts - 1));
-  u64 limit_of_all = theirs->limit;
+          for (int c = 0; c < parts; ++c) at[c] = above[c] + o <= k ? cluster.map_shared_rank(&sc, c)->sel[above[c] + o - 1] : 0;
 #pragma unroll
-  for (int o = parts / 2; o; o >>= 1) {
-    const u64 other = __shfl_xor_sync(0xffffffffu, limit_of_all, o);
-    limit_of_all = other > limit_of_all ? other : limit_of_all;
-  }
-  if (limit_of_all == 0) break;
-  int above = 0;
-  for (int o = first_o; o; o >>= 1) above += above + o <= k && theirs->sel[above + o - 1] > limit_of_all ? o : 0;
+          for (int c = 0; c < parts; ++c) above[c] += at[c] > own_key ? o : 0;
+        }
+        rank = 0;
 #pragma unroll
-  for (int o = parts / 2; o; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-  if (above >= k) break;
-  cluster.sync();  // all have read the lists that are made anew
-  }
+        for (int c = 0; c < parts; ++c) rank += above[c];
+      }
+      // Nothing is missing if k entries lie above every part's limit (lane c counts part c's).
+      const Scratch* theirs = cluster.map_shared_rank(&sc, lane & (parts - 1));
+      u64 limit_of_all = theirs->limit;
+#pragma unroll
+      for (int o = parts / 2; o; o >>= 1) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, limit_of_all, o);
+        limit_of_all = other > limit_of_all ? other : limit_of_all;
+      }
+      if (limit_of_all == 0) break;
+      int above = 0;
+      for (int o = first_o; o; o >>= 1) above += above + o <= k && theirs->sel[above + o - 1] > limit_of_all ? o : 0;
+#pragma unroll
+      for (int o = parts / 2; o; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+      if (above >= k) break;
+      cluster.sync();  // all have read the lists that are made anew
+    }
   }
   if (tid < kept && rank < k) {
     K::store(values, row * k + rank, static_cast<uint32_t>(own_key >> 32));

@@ -90,9 +90,10 @@ template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
 // One CTA's share [v0, v1) of the row.  16-byte loads where the three rows reach a
 // 16-byte boundary at the same element, single elements elsewhere (rows of an odd
 // vocabulary differ).  256 sequences x 5 drafts of 151936 fp32, 71 us at the copy rate:
-// 73.5 us in vectors, two in flight per row and thread so that four CTAs fit an SM
-// (four in flight, two CTAs: 114); of 151935 in single elements 87; with a division for
-// every element 155.
+// 72 us in vectors, two in flight per row and thread so that four CTAs fit an SM (four
+// in flight, two CTAs: 114); of 151935 in single elements 84; with a division for every
+// element 155.  One sequence takes 8 us, most of it the dependent loads of the acceptance
+// test and the exchange.
 template <typename T, bool DRAFT, int THREADS>
 __device__ __forceinline__ void scan(const T* p, const T* q, int hot, const float* e, int v0, int v1, Best& best) {
   using V = Vec<T>;
