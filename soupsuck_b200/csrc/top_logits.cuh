@@ -13,16 +13,16 @@
 //     memory, which is sorted out when the row has been read.
 // The threshold is a guess.  The 32 streams of a CTA (warp, vector) lie side by side in
 // the row, so the first round is an even sample of it; with s of n elements sampled, a
-// threshold that k s / n + 2.5 sqrt(k s / n) + 3 of them pass (taken from the threads'
-// maxima) leaves a few times k candidates and almost never fewer than k.  Where it does leave fewer, or the
-// list overflows (a row of equal or masked logits; where a cluster shares a row, where
+// threshold that k s / n + 2.5 to 5 sqrt(k s / n) + 3 of them pass (taken from the
+// threads' maxima) leaves a few times k candidates and seldom fewer than k.  Where it does
+// leave fewer, or the list overflows (a row of equal or masked logits; where a cluster shares a row, where
 // fewer than k of all parts' candidates lie above each part's threshold), the row is read
 // again with the
 // threshold that cannot fail: the k-th largest of the threads' maxima over a first chunk
 // in index order, raised to the k-th of all so far whenever the candidates have doubled;
 // the list then holds a whole chunk and is worked off at its end, so any row is handled.
 //
-// Measured, k = 64 (copy rate in brackets): 3300 rows of 151936 fp16 200 us (154; the safe
+// Measured, k = 64 (copy rate in brackets): 3300 rows of 151936 fp16 203 us (154; the safe
 // form alone 259, taking the vectors apart in the loop instead of listing them 703), fp32
 // about 330 (307), one row 10.  What bounds it: for 16-bit logits instruction issue and the
 // exponentials' unit, each about two thirds busy; for fp32 memory; for one row the chain of
@@ -378,7 +378,7 @@ __device__ __forceinline__ void rank_runs(int n, const Scratch& sc, F emit) {
 // nothing for a second attempt and needs fewer registers).
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(const T* __restrict__ logits, int64_t v, int64_t pitch,
-                                                          int k, float scale, float inv_tau, void* __restrict__ values,
+                                                          int k, float slack, float scale, float inv_tau, void* __restrict__ values,
                                                           int64_t* __restrict__ indices, float* __restrict__ lse) {
   using K = Kind<T>;
   constexpr int kBits = 8 * sizeof(T);
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, PARTS > 1 ? 3 : kPerSm) top_kernel(c
     // `want` elements of the sample above the threshold; as they fall into the threads at
     // random, so many threads' maxima are above it too.  (k maxima would never fail.)
     const float share = static_cast<float>(k) / max(rounds * parts, 1);
-    const float want = share + 2.5f * sqrtf(share) + 3.0f;
+    const float want = share + slack * sqrtf(share) + 3.0f;
     const float groups = static_cast<float>(max(min(kThreads, w1 - w0), 1));
     const int r = min(k, static_cast<int>(groups * (1.0f - __expf(-want / groups))) + 1);
     threshold(left > 0, r);
@@ -747,6 +747,18 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
          v / (parts * 2) >= (rows * parts * 2 <= sms ? chunk / 2 : 2 * chunk)) {
     parts *= 2;
   }
+  // How far the guess stays on the safe side, in standard deviations of the sample's count.
+  // While every row is resident, one that is read again is the whole call's time: 592 rows
+  // of 32001 bf16, k = 200, take 31.1 us at 2.5 and 24.6 at 4 (means of 16 inputs); 37 rows,
+  // whose parts are judged together, took 21 us at 2.5 for 6 of 32 inputs and 10.6 at 5 for
+  // all.  With more rows the others hide part of it and fewer candidates count for more:
+  // fp16, 2.5 against 4, 1000 rows of 151936 73 and 80 us, 2000 rows 129 and 137, 3300 203
+  // and 210; but only where the sample holds few of the k, so that the constant 3 is most of
+  // the margin (bf16: 16 of them, 2000 rows of 32001, k = 64, 49 and 51; 50 of them, 1000
+  // rows of 32001, k = 200, 46 and 40).  (It costs where the guess would have held: 300
+  // rows of 151936 34.3 and 35.7.)
+  const bool spare = rows > static_cast<int64_t>(kPerSm) * sms && k * chunk <= 32 * v;
+  const float slack = spare ? 2.5f : parts > 1 ? 5.0f : 4.0f;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
   cfg.blockDim = dim3(kThreads);
@@ -758,7 +770,7 @@ int launch(const void* logits, int64_t rows, int64_t v, int64_t pitch, int k, fl
   cfg.attrs = attr;
   cfg.numAttrs = parts > 1 ? 1 : 0;
   auto kern = parts == 1 ? top_kernel<T, 1> : parts == 2 ? top_kernel<T, 2> : parts == 4 ? top_kernel<T, 4> : top_kernel<T, 8>;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(logits), v, pitch, k,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(logits), v, pitch, k, slack,
                                            1.4426950408889634f / temperature, 1.0f / temperature, values, indices, lse);
   if (e != cudaSuccess) return fail(SB_ECUDA, std::string("top_kernel: ") + cudaGetErrorString(e));
   count_launch();
