@@ -694,6 +694,9 @@ int forward(int64_t t, int64_t h, const uint16_t* weight, int64_t v, int k, floa
     // V = 20000, tau = 2 the error is then 0.7 to 1.2 times that of products and sums in
     // fp32 throughout (in one run 2.2 times at H = 128 and 250); shorter runs are more
     // exact and slower (H = 1536: three k-blocks 1.22 against 1.09 ms at T = 3300).
+    // Of 1 to 48 rows the error is 0.71 times fp32's on average (40 inputs; single ones 4
+    // times over 1.5, 23 times below 1 / 1.5); three k-blocks 0.43, for 3 to 8 % of the time
+    // at 48 rows.
     p.seg = (p.k_blocks + 3) / 4;
     if (p.seg > 6) p.seg = 6;
     p.scale = scale;
